@@ -164,7 +164,7 @@ def _lookup(s):
 def _sort(s):
     keys, order = torch.sort(_keys(s["index"], s["case"]["codes"]), stable=True)
     offsets = torch.searchsorted(keys, torch.arange(s["case"]["codes"] + 1, device=keys.device))
-    return order.int(), offsets.int()
+    return order.int(), keys.int(), offsets.int()
 
 
 def _grad(s):
@@ -235,7 +235,7 @@ def work(case):
         return {"bytes": 2 * size, "flops": 3 * sum(lengths)}
     n, codes = case["n"], case["codes"]
     if op == "sort":
-        return {"bytes": n * (SIZE[case["index"]] + 4) + 4 * (codes + 1), "flops": 0}
+        return {"bytes": n * (SIZE[case["index"]] + 8) + 4 * (codes + 1), "flops": 0}
     used = min(n, codes) if op == "lookup" else codes
     return {"bytes": n * SIZE[case["index"]] + used * case["d"] * SIZE[case["table"]] + n * case["d"] * SIZE[case["rows"]],
             "flops": n * case["d"]}
@@ -253,9 +253,10 @@ def exact(case, seed):
         out[valid] = host(s["table"])[index[valid]] * s["scale"]
         return out
     if op == "sort":
-        order = np.argsort(np.where(valid, index, codes), kind="stable")
+        keys = np.where(valid, index, codes)
+        order = np.argsort(keys, kind="stable")
         counts = np.bincount(index[valid], minlength=codes)
-        return order.astype(np.int32), np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
+        return order.astype(np.int32), keys[order].astype(np.int32), np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
     if op == "grad":
         grad = host(s["grad"])[valid]
         return np.stack([np.bincount(index[valid], weights=grad[:, j], minlength=codes) for j in range(case["d"])], axis=1) * s["scale"]
