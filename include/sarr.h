@@ -201,6 +201,112 @@ int sarr_adam_step_ranges(int n_ranges, const int64_t *range_begin, const int64_
                           const float *grad, float *exp_avg, float *exp_avg_sq, float beta1,
                           float beta2, float eps, int64_t step, sarr_stream_t stream);
 
+/* Element types of the codebook and gradient-clipping entry points. */
+#define SARR_F32 0
+#define SARR_BF16 1
+#define SARR_F16 2
+
+/*
+ * Codebook rows: parameter rows (SH) taken from a table of `codes` rows that
+ * the Gaussians share, by index (an embedding lookup). No reference
+ * counterpart; the reference keeps 16 SH coefficients for every Gaussian.
+ *   rows[i,:] = scale * table[index[i],:]   for 0 <= index[i] < codes,
+ *   rows[i,:] = 0                           for any other index (no code).
+ *   index  [n], index_bits 32 or 64; table [codes, cols] in table_type, rows
+ *          [n, cols] in rows_type (table_type or SARR_F32), both with a row
+ *          stride in elements >= cols; the product is formed in 32 bits and
+ *          rounded once. rows must not overlap table. cols <= 2^22.
+ */
+int sarr_codebook_lookup(int64_t n, int64_t codes, int64_t cols, const void *index, int index_bits,
+                         const void *table, int table_type, int64_t table_stride, float scale,
+                         void *rows, int rows_type, int64_t rows_stride, sarr_stream_t stream);
+
+/*
+ * The Gaussians in the stable order of their codes, for sarr_codebook_grad:
+ *   order        [n] int32: the Gaussian at each place; those without a code
+ *                (index outside [0, codes)) come last, in their order too,
+ *   sorted_codes [n] int32: the code at each place, `codes` for none,
+ *   offsets      [codes + 1] int32: code c has places offsets[c] ..
+ *                offsets[c+1] - 1; offsets[codes] Gaussians have a code.
+ * n and codes below 2^31 - 2^19. Deterministic. The workspace
+ * (sarr_codebook_sort_workspace_size) is not needed after the call; the order
+ * may be kept as long as the index stays the same.
+ */
+int sarr_codebook_sort_workspace_size(int64_t n, int64_t codes, size_t *bytes);
+int sarr_codebook_sort(int64_t n, int64_t codes, const void *index, int index_bits, int32_t *order,
+                       int32_t *sorted_codes, int32_t *offsets, void *ws, size_t ws_bytes,
+                       sarr_stream_t stream);
+
+/*
+ * The gradient of sarr_codebook_lookup with respect to the table, from the
+ * order that sarr_codebook_sort gave:
+ *   grad_table[c,:] = scale * sum of grad_rows[i,:] over the Gaussians i of
+ *   code c, zeros where there are none (every row of grad_table is written).
+ *   grad_rows [n, cols] in rows_type; grad_table [codes, cols] in table_type
+ *   (the types are equal or one of them is SARR_F32), both with a row stride in
+ *   elements >= cols. Sums are kept in 32 bits and rounded once, in an order
+ *   that depends on the sizes and the codes only, so the result is reproducible.
+ *   order, sorted_codes and offsets must be what sarr_codebook_sort wrote for
+ *   the same n and codes.
+ */
+int sarr_codebook_grad_workspace_size(int64_t n, int64_t cols, size_t *bytes);
+int sarr_codebook_grad(int64_t n, int64_t codes, int64_t cols, const void *grad_rows, int rows_type,
+                       int64_t rows_stride, const int32_t *order, const int32_t *sorted_codes,
+                       const int32_t *offsets, float scale, void *grad_table, int table_type,
+                       int64_t table_stride, void *ws, size_t ws_bytes, sarr_stream_t stream);
+
+/* Global norms of a list of gradients: the 2-norm or the largest |element|. */
+#define SARR_NORM_2 0
+#define SARR_NORM_INF 1
+
+/*
+ * The norm of the elements of all n_tensors gradients together
+ * (torch.nn.utils.clip_grad_norm_'s total norm), written to norm_out (one
+ * float on the device). grads, counts and types are host arrays: the device
+ * pointer, the number of elements (contiguous memory) and the SARR_F32 /
+ * SARR_BF16 / SARR_F16 type of each tensor; types may be mixed. Squares are
+ * summed in 64 bits (no overflow or underflow of a square) in a fixed order.
+ * A NaN anywhere makes the norm NaN. An empty list has norm 0. Workspace:
+ * sarr_grad_norm_workspace_size. No reference counterpart (the reference
+ * trains without clipping).
+ */
+int sarr_grad_norm_workspace_size(int n_tensors, size_t *bytes);
+int sarr_grad_norm(int n_tensors, const void *const *grads, const int64_t *counts,
+                   const int32_t *types, int norm_kind, float *norm_out, void *ws, size_t ws_bytes,
+                   sarr_stream_t stream);
+
+/*
+ * Clips the gradients by their global norm N:
+ *   outs[t][j] = c * grads[t][j],  c = min(1, max_norm / (N + 1e-6)),
+ * c formed in 64 bits and rounded to 32, the product rounded once to outs'
+ * type. outs (host array of device pointers) may be grads itself (in place;
+ * nothing is rewritten where c = 1); otherwise no destination may share memory
+ * with another destination or with another tensor's gradient (checked:
+ * SARR_ERR_ARG). out_types: host array, each the gradient's type or SARR_F32;
+ * NULL for the gradients' own types. norm_out may be NULL. A NaN norm makes
+ * every output NaN and an infinite one makes c = 0, as
+ * torch.nn.utils.clip_grad_norm_ does. Workspace: sarr_grad_norm_workspace_size.
+ */
+int sarr_clip_grads(int n_tensors, const void *const *grads, const int64_t *counts,
+                    const int32_t *types, void *const *outs, const int32_t *out_types, int norm_kind,
+                    double max_norm, float *norm_out, void *ws, size_t ws_bytes,
+                    sarr_stream_t stream);
+
+/*
+ * sarr_adam_step_ranges with clipped gradients: the 2-norm N of the gradients
+ * of all the ranges together, then torch.optim.Adam's update of every range
+ * with c * g in the place of the gradient g (c as in sarr_clip_grads; the
+ * gradients are not rewritten). Up to 64 disjoint ranges (host arrays as in
+ * sarr_adam_step_ranges, range_lr in double); betas, eps and learning rates in
+ * double as torch holds them. norm_out (device float) may be NULL. Workspace:
+ * sarr_grad_norm_workspace_size(64).
+ */
+int sarr_adam_step_clipped(int n_ranges, const int64_t *range_begin, const int64_t *range_end,
+                           const int64_t *grad_begin, const double *range_lr, float *param,
+                           const float *grad, float *exp_avg, float *exp_avg_sq, double beta1,
+                           double beta2, double eps, int64_t step, double max_norm, float *norm_out,
+                           void *ws, size_t ws_bytes, sarr_stream_t stream);
+
 /*
  * Densification and pruning (GaussianModel.densify_and_prune,
  * gaussian_model.py:433-566) in two calls, with a host decision between them

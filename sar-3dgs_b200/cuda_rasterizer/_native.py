@@ -90,7 +90,21 @@ def _declare(L):
     L.sarr_densify_workspace_size.argtypes = [I64, ctypes.POINTER(SZ)]
     L.sarr_densify_flags.argtypes = [I64, P, P, P, F, F, F, F, P, P, SZ, P]
     L.sarr_densify_apply.argtypes = [I64, P, P, P, P, P, I, P, P, I, I, P, P, P, P, P, P, SZ, P]
-    for name in ("sarr_workspace_size", "sarr_state_size", "sarr_forward", "sarr_backward",
+    D = ctypes.c_double
+    SZP = ctypes.POINTER(SZ)
+    L.sarr_codebook_lookup.argtypes = [I64, I64, I64, P, I, P, I, I64, F, P, I, I64, P]
+    L.sarr_codebook_sort_workspace_size.argtypes = [I64, I64, SZP]
+    L.sarr_codebook_sort.argtypes = [I64, I64, P, I, P, P, P, P, SZ, P]
+    L.sarr_codebook_grad_workspace_size.argtypes = [I64, I64, SZP]
+    L.sarr_codebook_grad.argtypes = [I64, I64, I64, P, I, I64, P, P, P, F, P, I, I64, P, SZ, P]
+    L.sarr_grad_norm_workspace_size.argtypes = [I, SZP]
+    L.sarr_grad_norm.argtypes = [I, P, P, P, I, P, P, SZ, P]
+    L.sarr_clip_grads.argtypes = [I, P, P, P, P, P, I, D, P, P, SZ, P]
+    L.sarr_adam_step_clipped.argtypes = [I, P, P, P, P, P, P, P, P, D, D, D, I64, D, P, P, SZ, P]
+    for name in ("sarr_codebook_lookup", "sarr_codebook_sort_workspace_size", "sarr_codebook_sort",
+                 "sarr_codebook_grad_workspace_size", "sarr_codebook_grad",
+                 "sarr_grad_norm_workspace_size", "sarr_grad_norm", "sarr_clip_grads",
+                 "sarr_adam_step_clipped", "sarr_workspace_size", "sarr_state_size", "sarr_forward", "sarr_backward",
                  "sarr_backward_scatter",
                  "sarr_debug_preprocess", "sarr_debug_tile_lists", "sarr_check_device_errors",
                  "sarr_debug_tile_rect", "sarr_gaussian_params", "sarr_loss_workspace_size",

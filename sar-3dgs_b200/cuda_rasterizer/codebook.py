@@ -1,0 +1,200 @@
+"""Codebook rows: Gaussians whose parameter rows (the SH coefficients, 16 of a
+Gaussian's 20 trained floats) come from a table that they share, by index.
+
+    rows = lookup(table, index, scale)        # rows[i] = scale * table[index[i]]
+
+`lookup` is differentiable with respect to the table. Its gradient sums the
+rows' gradients of every code in the order of the Gaussians: `gradient` sorts
+the index and sums, `sort_by_code` and `gradient_sorted` are its two halves for
+a caller whose index stays the same over many steps (ViewParallelTrainer with
+`sh_index`). A Gaussian whose index is outside [0, codes) has no code: its row
+is zeros and its gradient reaches no code.
+
+Tables and rows are float32, bfloat16 or float16 CUDA tensors (rows in the
+table's type or float32); indexes int32 or int64. Products and sums are formed
+in 32 bits and rounded once; results are bitwise reproducible. No counterpart
+in the reference, which keeps all SH coefficients of every Gaussian.
+"""
+import ctypes
+from typing import NamedTuple, Optional
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _native
+
+__all__ = ["SortedCodes", "lookup", "sort_by_code", "gradient", "gradient_sorted"]
+
+_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_INDEX_BITS = {torch.int32: 32, torch.int64: 64}
+
+
+class SortedCodes(NamedTuple):
+    """The Gaussians in the stable order of their codes (sarr_codebook_sort)."""
+    order: torch.Tensor    # int32 [n]: the Gaussian at each place, those without a code last
+    codes: torch.Tensor    # int32 [n]: the code at each place, `codes` for none
+    offsets: torch.Tensor  # int32 [codes + 1]: the first place of each code
+
+
+def _matrix(t, name):
+    """(tensor, row stride) of a [rows, cols] matrix of a supported type."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if not t.is_cuda:
+        raise RuntimeError(f"{name} must be a CUDA tensor (there is no CPU path)")
+    if t.dtype not in _TYPES:
+        raise RuntimeError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
+    if t.dim() != 2:
+        raise RuntimeError(f"{name} must be a matrix, got shape {tuple(t.shape)}")
+    rows, cols = t.shape
+    if (cols > 1 and t.stride(1) != 1) or (rows > 1 and t.stride(0) < cols):
+        t = t.contiguous()
+    return t, max(t.stride(0), cols) if rows > 1 else cols
+
+
+def _index(index, name="index"):
+    if not isinstance(index, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if not index.is_cuda:
+        raise RuntimeError(f"{name} must be a CUDA tensor (there is no CPU path)")
+    if index.dtype not in _INDEX_BITS:
+        raise RuntimeError(f"{name} must be int32 or int64, got {index.dtype}")
+    return index.reshape(-1).contiguous()
+
+
+def _same_device(dev, **tensors):
+    for name, t in tensors.items():
+        if t.device != dev:
+            raise RuntimeError(f"{name} is on {t.device}, expected {dev}")
+
+
+def _out_type(dtype, allowed, what):
+    if dtype not in allowed:
+        raise RuntimeError(f"{what} must be one of {[str(d) for d in allowed]}, got {dtype}")
+    return dtype
+
+
+def _size(fn, *args):
+    out = ctypes.c_size_t()
+    _native._check(fn(*args, ctypes.byref(out)), fn.__name__)
+    return out.value
+
+
+def _lookup(table, index, scale, dtype, out=None):
+    table, stride = _matrix(table, "table")
+    shape = index.shape
+    index = _index(index)
+    dev = table.device
+    _same_device(dev, index=index)
+    dtype = _out_type(dtype or table.dtype, (table.dtype, torch.float32), "dtype")
+    codes, cols = table.shape
+    n = index.numel()
+    if out is None:
+        rows = torch.empty((n, cols), dtype=dtype, device=dev)
+        rows_stride = cols
+    else:
+        rows, rows_stride = _matrix(out, "out")
+        if rows is not out or rows.dtype != dtype or rows.shape != (n, cols):
+            raise RuntimeError(f"out must be a {dtype} matrix of {n} x {cols} with contiguous rows")
+        _same_device(dev, out=rows)
+    with torch.cuda.device(dev):
+        _native._check(_native.lib().sarr_codebook_lookup(
+            n, codes, cols, index.data_ptr(), _INDEX_BITS[index.dtype], table.data_ptr(),
+            _TYPES[table.dtype], stride, float(scale), rows.data_ptr(), _TYPES[dtype], rows_stride,
+            _native._stream(dev)), "sarr_codebook_lookup")
+    return rows if out is not None else rows.view(*shape, cols)
+
+
+def sort_by_code(index: torch.Tensor, codes: int) -> SortedCodes:
+    """The stable order of the Gaussians by code (`index` flattened)."""
+    index = _index(index)
+    dev, n, codes = index.device, index.numel(), int(codes)
+    L = _native.lib()
+    with torch.cuda.device(dev):
+        ws = torch.empty(_size(L.sarr_codebook_sort_workspace_size, n, codes), dtype=torch.uint8, device=dev)
+        order = torch.empty(n, dtype=torch.int32, device=dev)
+        sorted_codes = torch.empty(n, dtype=torch.int32, device=dev)
+        offsets = torch.empty(codes + 1, dtype=torch.int32, device=dev)
+        _native._check(L.sarr_codebook_sort(
+            n, codes, index.data_ptr(), _INDEX_BITS[index.dtype], order.data_ptr(),
+            sorted_codes.data_ptr(), offsets.data_ptr(), ws.data_ptr(), ws.numel(),
+            _native._stream(dev)), "sarr_codebook_sort")
+    return SortedCodes(order, sorted_codes, offsets)
+
+
+def gradient_sorted(grad_rows: torch.Tensor, sorted_codes: SortedCodes, scale: float = 1.0,
+                    dtype: Optional[torch.dtype] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The table's gradient [codes, cols] from the rows' gradients [n, cols] and
+    the order that sort_by_code gave for their index. `dtype`: the result's type
+    (the rows' type by default; float32, or any of the three for float32 rows);
+    `out`: a matrix to write it into (its rows may be strided)."""
+    rows, rows_stride = _matrix(grad_rows, "grad_rows")
+    n, cols = rows.shape
+    order, places, offsets = sorted_codes
+    dev = rows.device
+    for name, t in (("order", order), ("codes", places), ("offsets", offsets)):
+        if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous():
+            raise RuntimeError(f"sorted_codes.{name} must be a contiguous int32 vector")
+        _same_device(dev, **{f"sorted_codes.{name}": t})
+    if order.numel() != n or places.numel() != n or offsets.numel() < 1:
+        raise RuntimeError(f"sorted_codes is of {order.numel()} Gaussians, grad_rows of {n}")
+    codes = offsets.numel() - 1
+    if out is None:
+        dtype = dtype or rows.dtype
+    elif dtype is not None and dtype != out.dtype:
+        raise RuntimeError(f"out is {out.dtype}, dtype {dtype}")
+    else:
+        dtype = out.dtype
+    allowed = tuple(_TYPES) if rows.dtype == torch.float32 else (rows.dtype, torch.float32)
+    dtype = _out_type(dtype, allowed, "dtype")
+    if out is None:
+        table = torch.empty((codes, cols), dtype=dtype, device=dev)
+        stride = cols
+    else:
+        table, stride = _matrix(out, "out")
+        if table is not out or table.shape != (codes, cols):
+            raise RuntimeError(f"out must be a matrix of {codes} x {cols} with contiguous rows")
+        _same_device(dev, out=table)
+    L = _native.lib()
+    with torch.cuda.device(dev):
+        ws = torch.empty(_size(L.sarr_codebook_grad_workspace_size, n, cols), dtype=torch.uint8, device=dev)
+        _native._check(L.sarr_codebook_grad(
+            n, codes, cols, rows.data_ptr(), _TYPES[rows.dtype], rows_stride, order.data_ptr(),
+            places.data_ptr(), offsets.data_ptr(), float(scale), table.data_ptr(), _TYPES[dtype], stride,
+            ws.data_ptr(), ws.numel(), _native._stream(dev)), "sarr_codebook_grad")
+    return table
+
+
+def gradient(grad_rows: torch.Tensor, index: torch.Tensor, codes: int, scale: float = 1.0,
+             dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """The table's gradient [codes, cols] of lookup(table, index, scale) from the
+    rows' gradients [*index.shape, cols]."""
+    rows = grad_rows.reshape(-1, grad_rows.shape[-1]) if grad_rows.dim() != 2 else grad_rows
+    if rows.shape[0] != index.numel():
+        raise RuntimeError(f"grad_rows has {rows.shape[0]} rows, index {index.numel()} elements")
+    return gradient_sorted(rows, sort_by_code(index, codes), scale, dtype)
+
+
+class _Lookup(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, table, index, scale, dtype):
+        rows = _lookup(table.detach(), index, scale, dtype)
+        ctx.save_for_backward(index)
+        ctx.scale, ctx.codes, ctx.dtype = scale, table.shape[0], table.dtype
+        return rows
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        (index,) = ctx.saved_tensors
+        return gradient(grad, index, ctx.codes, ctx.scale, ctx.dtype), None, None, None
+
+
+def lookup(table: torch.Tensor, index: torch.Tensor, scale: float = 1.0,
+           dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """rows[i] = scale * table[index[i]] ([*index.shape, cols]; zeros where
+    index[i] is outside [0, codes)), in `dtype` (the table's type by default, or
+    float32), with its gradient with respect to the table."""
+    if isinstance(table, torch.Tensor) and table.requires_grad and torch.is_grad_enabled():
+        return _Lookup.apply(table, index, scale, dtype)
+    return _lookup(table, index, scale, dtype)
