@@ -135,25 +135,47 @@ class ViewParallelTrainer:
     Learning rates per group follow train.py:429-435 (lr for means and
     opacity, lr / 100 for SH). Every rank must call step() the same number of
     times with the same number of views (the all-reduces are collective).
+
+    Two options without a counterpart in the reference:
+
+    sh_index [n]: the SH rows come from a codebook that the Gaussians share
+    (cuda_rasterizer.codebook). `sh` is then the table [codes, K], which is
+    what is trained (the flat buffer is means | logits | table), and Gaussian
+    i renders sh_scale * sh[sh_index[i]] (zeros for index -1). The index is
+    fixed for the trainer's life, so it is sorted once; each step looks the
+    rows up, and sums their gradients over the codes after the last bucket's
+    rows (one all-reduce more, of the table).
+
+    max_grad_norm: each step's gradients (summed over the ranks) are clipped
+    to this 2-norm over all parameters inside the Adam update
+    (sarr_adam_step_clipped); every update then waits for all the
+    all-reduces, since the norm is over all buckets. `grad_norm` holds the
+    last update's norm before clipping (device scalar).
     """
 
     def __init__(self, means, scales_log, rotations, opacity_logits, sh, lr=1e-3, group=None,
                  buckets=4, l1_weight=1.0, ssim_weight=0.2, window_size=5, betas=(0.9, 0.999),
-                 eps=1e-8, distributed=True):
+                 eps=1e-8, distributed=True, sh_index=None, sh_scale=1.0, max_grad_norm=None):
         from . import _native
         self._N = _native
         dev = means.device
         n, k = means.shape[0], sh.shape[1]
+        if max_grad_norm is not None and not float(max_grad_norm) >= 0.0:
+            raise ValueError(f"max_grad_norm must be >= 0, got {max_grad_norm}")
         self.n, self.k, self.device = n, k, dev
         self.group = group
         # distributed=False: a single-process trainer even inside a process group
         self.world = (dist.get_world_size(group) if distributed and dist.is_available()
                       and dist.is_initialized() else 1)
-        total = n * (4 + k)
+        self.sh_index, self.sh_scale = None, float(sh_scale)
+        if sh_index is not None:
+            self._set_index(sh_index, sh.shape[0])
+        sh_rows = n if sh_index is None else sh.shape[0]  # rows of the trained SH parameter
+        total = 4 * n + k * sh_rows
         self.param = torch.empty(total, dtype=torch.float32, device=dev)
         self.means = self.param[:3 * n].view(n, 3)
         self.logits = self.param[3 * n:4 * n]
-        self.sh = self.param[4 * n:].view(n, k)
+        self.sh = self.param[4 * n:].view(sh_rows, k)
         self.means.copy_(means)
         self.logits.copy_(opacity_logits.reshape(n))
         self.sh.copy_(sh)
@@ -173,8 +195,20 @@ class ViewParallelTrainer:
         self.grad = torch.zeros_like(self.param)
         self.gparts = []  # per bucket: (offset, means [nb,3], logits [nb], SH [nb,K], whole)
         o = 0
+        # with a codebook the SH rows and their gradients are scratch, and the
+        # table's gradient is the last bucket
+        self.sh_rows = self.g_sh_rows = self.g_table = None
+        if self.sh_index is not None:
+            self.sh_rows = torch.empty((n, k), dtype=torch.float32, device=dev)
+            self.g_sh_rows = torch.empty((n, k), dtype=torch.float32, device=dev)
+            self.g_table = self.grad[4 * n:].view(sh_rows, k)
         for g0, g1 in self.bounds:
             nb = g1 - g0
+            if self.sh_index is not None:
+                self.gparts.append((o, self.grad[o:o + 3 * nb].view(nb, 3), self.grad[o + 3 * nb:o + 4 * nb],
+                                    self.g_sh_rows[g0:g1], self.grad[o:o + 4 * nb]))
+                o += 4 * nb
+                continue
             self.gparts.append((o, self.grad[o:o + 3 * nb].view(nb, 3), self.grad[o + 3 * nb:o + 4 * nb],
                                 self.grad[o + 4 * nb:o + (4 + k) * nb].view(nb, k),
                                 self.grad[o:o + (4 + k) * nb]))
@@ -188,6 +222,26 @@ class ViewParallelTrainer:
         self.sh_active = k
         self._buf_key = None
         self._args = None
+        self.max_grad_norm = None if max_grad_norm is None else float(max_grad_norm)
+        self.grad_norm = None
+        if self.max_grad_norm is not None:
+            from . import clipping
+            if 3 * len(self.bounds) + 1 > clipping.MAX_RANGES:
+                raise ValueError(f"at most {(clipping.MAX_RANGES - 1) // 3} buckets with max_grad_norm")
+            self.grad_norm = torch.zeros((), dtype=torch.float32, device=dev)
+            self.norm_ws = clipping._workspace(clipping.MAX_RANGES, dev)
+
+    def _set_index(self, sh_index, codes):
+        """The codebook index (checked and sorted once)."""
+        from . import codebook
+        if sh_index.dim() != 1 or sh_index.shape[0] != self.n:
+            raise ValueError(f"sh_index must have N={self.n} elements, got shape {tuple(sh_index.shape)}")
+        if sh_index.dtype not in (torch.int32, torch.int64):
+            raise ValueError(f"sh_index must be int32 or int64, got {sh_index.dtype}")
+        if self.n and not (-1 <= int(sh_index.min()) and int(sh_index.max()) < codes):
+            raise ValueError(f"sh_index must be -1 or a row of the table of {codes}")
+        self.sh_index = sh_index.detach().to(device=self.device, dtype=torch.int32).clone()
+        self.sh_order = codebook.sort_by_code(self.sh_index, codes)
 
     def _buffers(self, views):
         """Buffers and C-call arguments for this views list (rebuilt when the
@@ -227,12 +281,20 @@ class ViewParallelTrainer:
             for (g0, g1), (o, gm, gl, gsh, _) in zip(self.bounds, self.gparts):
                 nb = g1 - g0
                 segs = flat_segments(self.n, self.k, g0, g1)
-                ranges.append(((ctypes.c_int64 * 3)(*[x[0] for x in segs]),
-                               (ctypes.c_int64 * 3)(*[x[1] for x in segs]),
-                               (ctypes.c_int64 * 3)(o, o + 3 * nb, o + 4 * nb),
-                               (ctypes.c_float * 3)(*[self.group_lr[x[2]] for x in segs])))
+                if self.sh_index is not None:
+                    segs = segs[:2]
+                ranges.append([(x[0], x[1], first, self.group_lr[x[2]])
+                               for x, first in zip(segs, (o, o + 3 * nb, o + 4 * nb))])
                 gptr.append((P(gm), P(gl), P(gsh)))
-            a["ranges"] = ranges
+            if self.sh_index is not None:
+                a["sh"] = P(self.sh_rows)
+                total = self.param.numel()
+                ranges.append([(4 * self.n, total, 4 * self.n, self.group_lr[2])])
+            # per bucket, as (begin, end, first gradient, lr) and as C arrays
+            a["flat_ranges"] = [r for bucket in ranges for r in bucket]
+            a["ranges"] = [(len(rs), *[(t * len(rs))(*[r[j] for r in rs]) for j, t in
+                                       enumerate((ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_float))])
+                           for rs in ranges]
             a["gptr"] = gptr
             self._args = a
         return self._args
@@ -258,6 +320,8 @@ class ViewParallelTrainer:
             N._check(L.sarr_gaussian_params(n, A["scales"], A["rotations"], A["cov6"], N.SARR_COV6,
                                             A["logits"], A["sigma"], st), "sarr_gaussian_params")
             ka = self.sh_active
+            if self.sh_index is not None:
+                self._lookup(ka)
             N._check(L.sarr_forward(vs, V, n, A["means"], A["cov6"], N.SARR_COV6, A["sigma"], A["sh"],
                                     k, ka, P(self.images), None, states, ws, wsb, st), "sarr_forward")
             l1w, ssw, win = self.loss_w
@@ -280,9 +344,12 @@ class ViewParallelTrainer:
                                                  gl, gsh, k, None, N.SARR_FLAG_RANGE_ROWS, ws, wsb,
                                                  st), "sarr_backward_scatter")
                 self.gparts[b][2].mul_(dsig[g0:g1])
-                if ka < k:
+                if ka < k and self.sh_index is None:
                     self.gparts[b][3][:, ka:].zero_()
                 works.append(self._allreduce_bucket(b))
+            if self.sh_index is not None:
+                self._table_gradient(ka)
+                works.append(self._allreduce_bucket(len(self.bounds)))
             if not update:
                 for w in (w for ws_ in works for w in ws_):
                     w.wait()
@@ -305,28 +372,54 @@ class ViewParallelTrainer:
             self.steps_done += 1
             self._update([], N._stream(self.device))
 
+    def _lookup(self, ka):
+        """The rendered SH rows: the first ka columns of the codebook's rows."""
+        from . import codebook
+        codebook._lookup(self.sh[:, :ka], self.sh_index, self.sh_scale, torch.float32, out=self.sh_rows[:, :ka])
+
+    def _table_gradient(self, ka):
+        from . import codebook
+        codebook.gradient_sorted(self.g_sh_rows[:, :ka], self.sh_order, self.sh_scale, out=self.g_table[:, :ka])
+        if ka < self.k:
+            self.g_table[:, ka:].zero_()
+
     def _allreduce_bucket(self, b):
+        """Bucket b's all-reduce; the one behind the Gaussians' is the table's."""
         if self.world == 1:
             return []
-        return [dist.all_reduce(self.gparts[b][4], group=self.group, async_op=True)]
+        part = self.gparts[b][4] if b < len(self.gparts) else self.grad[4 * self.n:]
+        return [dist.all_reduce(part, group=self.group, async_op=True)]
 
     def gradients(self):
         """The last step's gradients (summed over the ranks) in the parameter
-        layout: (means [n,3], opacity logits [n], SH [n,K])."""
+        layout: (means [n,3], opacity logits [n], SH [n,K] or, with a
+        codebook, its table's [codes,K])."""
+        if self.sh_index is not None:
+            return (torch.cat([p[1] for p in self.gparts]), torch.cat([p[2] for p in self.gparts]),
+                    self.g_table.clone())
         return (torch.cat([p[1] for p in self.gparts]), torch.cat([p[2] for p in self.gparts]),
                 torch.cat([p[3] for p in self.gparts]))
 
     def _update(self, works, st):
         """Each bucket's Adam update (one launch over its means, opacity and
-        SH ranges), queued behind its all-reduces."""
+        SH ranges), queued behind its all-reduces; with max_grad_norm one
+        update of all buckets behind all of them."""
         N = self._N
         L = N.lib()
         A = self._call_args()
         b1, b2 = self.betas
-        for i, (begin, end, gbegin, lr) in enumerate(A["ranges"]):
+        if self.max_grad_norm is not None:
+            from . import clipping
+            for w in (w for ws in works for w in ws):
+                w.wait()
+            clipping.adam_ranges_clipped((self.param, self.grad, self.exp_avg, self.exp_avg_sq), A["flat_ranges"],
+                                         self.steps_done, self.max_grad_norm, self.betas, self.eps, self.grad_norm,
+                                         self.norm_ws)
+            return
+        for i, (count, begin, end, gbegin, lr) in enumerate(A["ranges"]):
             for w in works[i] if works else []:
                 w.wait()  # the current stream waits for this bucket's all-reduce
-            N._check(L.sarr_adam_step_ranges(3, begin, end, gbegin, lr, A["param"], A["grad"],
+            N._check(L.sarr_adam_step_ranges(count, begin, end, gbegin, lr, A["param"], A["grad"],
                                              A["exp_avg"], A["exp_avg_sq"], float(b1), float(b2),
                                              float(self.eps), self.steps_done, st),
                      "sarr_adam_step_ranges")
@@ -335,7 +428,8 @@ class ViewParallelTrainer:
         """The step's collectives alone (the same buckets, back to back), for
         measuring their cost; a no-op on one rank."""
         if self.world > 1:
-            works = [w for b in range(len(self.bounds)) for w in self._allreduce_bucket(b)]
+            buckets = len(self.bounds) + (self.sh_index is not None)
+            works = [w for b in range(buckets) for w in self._allreduce_bucket(b)]
             for w in works:
                 w.wait()
 
@@ -373,7 +467,9 @@ class DensifyingTrainer:
     gradient) and training continues on a new ViewParallelTrainer over the new
     set; if it did not, Adam restarts from zero moments with this step's
     gradients. `history` records each densification as (iteration, n before,
-    clones, splits, prunes, n after).
+    clones, splits, prunes, n after). With a codebook (sh_index, a
+    ViewParallelTrainer option) clones and splits keep their Gaussian's code,
+    and the table goes on as it is.
     """
 
     def __init__(self, means, scales_log, rotations, opacity_logits, sh, lr=1e-3, group=None,
@@ -387,10 +483,10 @@ class DensifyingTrainer:
         self.sh_interval, self.max_sh_degree = sh_interval, max_sh_degree
         self.iteration = 0
         self.history = []
-        self.tr = self._trainer(means, scales_log, rotations, opacity_logits, sh)
+        self.tr = self._trainer(means, scales_log, rotations, opacity_logits, sh, self.trainer_kw.pop("sh_index", None))
 
-    def _trainer(self, means, scales_log, rotations, logits, sh):
-        return ViewParallelTrainer(means, scales_log, rotations, logits, sh, lr=self.lr,
+    def _trainer(self, means, scales_log, rotations, logits, sh, sh_index=None):
+        return ViewParallelTrainer(means, scales_log, rotations, logits, sh, lr=self.lr, sh_index=sh_index,
                                    group=self.group, buckets=self.buckets, **self.trainer_kw)
 
     @property
@@ -413,13 +509,18 @@ class DensifyingTrainer:
         from . import densify as DZ
         tr = self.tr
         grad_means = tr.gradients()[0]
-        out, counts = DZ.densify_and_prune_tensors(tr.means, tr.scales, tr.rotations, tr.logits, tr.sh,
+        # a codebook's index moves with its Gaussians as a row of one 32-bit
+        # word (densification only copies these rows)
+        rows = tr.sh if tr.sh_index is None else tr.sh_index.view(torch.float32).unsqueeze(1)
+        out, counts = DZ.densify_and_prune_tensors(tr.means, tr.scales, tr.rotations, tr.logits, rows,
                                                    grad_means, *self.thresholds, self.max_gaussians)
         clones, splits, prunes, new = counts
         n_before = tr.n
         if prunes == 0 and new == 0:
             tr.reset_optimizer()
             tr.apply_update()
-        else:
+        elif tr.sh_index is None:
             self.tr = self._trainer(*out)
+        else:
+            self.tr = self._trainer(*out[:4], tr.sh, out[4].view(torch.int32).reshape(-1))
         self.history.append((self.iteration, n_before, clones, splits, prunes, self.tr.n))
