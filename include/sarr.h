@@ -228,9 +228,9 @@ int sarr_codebook_lookup(int64_t n, int64_t codes, int64_t cols, const void *ind
  *   sorted_codes [n] int32: the code at each place, `codes` for none,
  *   offsets      [codes + 1] int32: code c has places offsets[c] ..
  *                offsets[c+1] - 1; offsets[codes] Gaussians have a code.
- * n and codes below 2^31 - 2^19. Deterministic. The workspace
- * (sarr_codebook_sort_workspace_size) is not needed after the call; the order
- * may be kept as long as the index stays the same.
+ * n and codes at most 2^31 - 1 - 2^19. Deterministic. The workspace
+ * (sarr_codebook_sort_workspace_size; NULL where that is 0 bytes) is not needed
+ * after the call; the order may be kept as long as the index stays the same.
  */
 int sarr_codebook_sort_workspace_size(int64_t n, int64_t codes, size_t *bytes);
 int sarr_codebook_sort(int64_t n, int64_t codes, const void *index, int index_bits, int32_t *order,
@@ -254,6 +254,16 @@ int sarr_codebook_grad(int64_t n, int64_t codes, int64_t cols, const void *grad_
                        int64_t rows_stride, const int32_t *order, const int32_t *sorted_codes,
                        const int32_t *offsets, float scale, void *grad_table, int table_type,
                        int64_t table_stride, void *ws, size_t ws_bytes, sarr_stream_t stream);
+
+/*
+ * sarr_codebook_sort and sarr_codebook_grad in one call, for an index that is
+ * used once; the order is kept in the workspace.
+ */
+int sarr_codebook_gradient_workspace_size(int64_t n, int64_t codes, int64_t cols, size_t *bytes);
+int sarr_codebook_gradient(int64_t n, int64_t codes, int64_t cols, const void *grad_rows, int rows_type,
+                           int64_t rows_stride, const void *index, int index_bits, float scale,
+                           void *grad_table, int table_type, int64_t table_stride, void *ws,
+                           size_t ws_bytes, sarr_stream_t stream);
 
 /* Global norms of a list of gradients: the 2-norm or the largest |element|. */
 #define SARR_NORM_2 0

@@ -39,9 +39,11 @@ void count_launches(int k);  // the library's launch counter (sarr_abi.cu)
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kPiece = 4096;        // elements of a piece: 16 per thread
-constexpr int kNormCtas = 148 * 4;  // the most CTAs (and partials) of one norm_kernel launch
-constexpr int kSmallList = 16, kLargeList = 512;  // tensors of one launch (kernel parameters)
+constexpr int kVecs = 4;                        // 16-byte loads of a thread for a piece, in flight together
+constexpr int kPieceBytes = kThreads * kVecs * 16;  // of the gradient
+constexpr int kNormCtas = 148 * 4;              // the most CTAs (and partials) of one norm_kernel launch
+constexpr int kClipCtas = 148 * 4, kAdamCtas = 148 * 4;
+constexpr int kSmallList = 16, kMediumList = 96, kLargeList = 512;  // tensors of one launch (kernel parameters)
 constexpr int kAdamRanges = 64;
 
 // One tensor of a list. Elements are numbered from the 16-byte boundary at or
@@ -152,24 +154,40 @@ __device__ __forceinline__ int64_t first_piece(const TensorList<kMax>& L, int t)
   return t > 0 ? L.e[t - 1].piece_end : 0;
 }
 
+// The elements of the 16 bytes at element i (numbered as in Entry) that belong to
+// the tensor, one by one.
 template <bool kInf>
-__device__ __forceinline__ double piece_norm(const Entry& E, int64_t at, double acc) {
-  const int per = E.type == SARR_F32 ? 4 : 8;  // elements of 16 bytes
-  const int64_t end = E.lead + E.count;
-  const char* base = static_cast<const char*>(E.in) - (int64_t)E.lead * (16 / per);
-  for (int v = threadIdx.x; v < kPiece / per; v += kThreads) {
-    const int64_t i = at + (int64_t)v * per;
-    if (i >= E.lead && i + per <= end) {
-      const uint4 q = *reinterpret_cast<const uint4*>(base + i * (16 / per));
-      float x[8];
-      unpack(q, E.type, x);
+__device__ __forceinline__ double ragged_norm(const Entry& E, int64_t i, int per, double acc) {
+  for (int k = 0; k < per; ++k)
+    if (i + k >= E.lead && i + k < E.lead + E.count)
+      acc = norm_add<kInf>(acc, load_as_float(E.in, E.type, i + k - E.lead));
+  return acc;
+}
+
+template <int kType, bool kInf>
+__device__ __forceinline__ double piece_norm(const Entry& E, int64_t piece, double acc) {
+  constexpr int kPer = kType == SARR_F32 ? 4 : 8;  // elements of 16 bytes
+  const int64_t at = piece * (kThreads * kVecs * kPer), end = E.lead + E.count;
+  const uint4* p = reinterpret_cast<const uint4*>(static_cast<const char*>(E.in) - E.lead * (16 / kPer)) + at / kPer;
+  uint4 q[kVecs];
+  if (at >= E.lead && at + kThreads * kVecs * kPer <= end) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k)
-        if (k < per) acc = norm_add<kInf>(acc, x[k]);
-    } else {
-      for (int k = 0; k < per; ++k)
-        if (i + k >= E.lead && i + k < end) acc = norm_add<kInf>(acc, load_as_float(E.in, E.type, i + k - E.lead));
+    for (int k = 0; k < kVecs; ++k) q[k] = p[k * kThreads + threadIdx.x];
+  } else {
+#pragma unroll
+    for (int k = 0; k < kVecs; ++k) {
+      const int64_t i = at + (int64_t)(k * kThreads + threadIdx.x) * kPer;
+      q[k] = make_uint4(0, 0, 0, 0);
+      if (i >= E.lead && i + kPer <= end) q[k] = p[k * kThreads + threadIdx.x];
+      else acc = ragged_norm<kInf>(E, i, kPer, acc);
     }
+  }
+#pragma unroll
+  for (int k = 0; k < kVecs; ++k) {
+    float x[8];
+    unpack(q[k], kType, x);
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) acc = norm_add<kInf>(acc, x[j]);
   }
   return acc;
 }
@@ -183,10 +201,18 @@ __global__ void __launch_bounds__(kThreads) norm_kernel(const __grid_constant__ 
   double acc = 0.0;
   if (p0 < p1) {
     int t = find_tensor(L, p0);
-    int64_t first = first_piece(L, t);
-    for (int64_t p = p0; p < p1; ++p) {
-      while (p >= L.e[t].piece_end) first = L.e[t++].piece_end;
-      acc = piece_norm<kInf>(L.e[t], (p - first) * kPiece, acc);
+    int64_t first = first_piece(L, t), p = p0;
+    while (p < p1) {
+      const Entry E = L.e[t];
+      const int64_t stop = min(p1, E.piece_end);
+      if (E.type == SARR_F32)
+        for (; p < stop; ++p) acc = piece_norm<SARR_F32, kInf>(E, p - first, acc);
+      else if (E.type == SARR_BF16)
+        for (; p < stop; ++p) acc = piece_norm<SARR_BF16, kInf>(E, p - first, acc);
+      else
+        for (; p < stop; ++p) acc = piece_norm<SARR_F16, kInf>(E, p - first, acc);
+      first = E.piece_end;
+      ++t;
     }
   }
   acc = block_join<kInf>(acc);
@@ -219,52 +245,71 @@ __device__ __forceinline__ float clip_coef(double norm, double max_norm) {
 // ---------------------------------------------------------------------------
 // clip
 // ---------------------------------------------------------------------------
-__device__ __forceinline__ void piece_clip(const Entry& E, int64_t at, float c) {
-  const int per = E.type == SARR_F32 ? 4 : 8;
-  const int64_t end = E.lead + E.count;
+template <int kOut>
+__device__ __forceinline__ void store_scaled(char* o, const float* x, int n, float c) {
+  uint32_t w[8];
+  if (kOut == SARR_F32) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (k < n) w[k] = __float_as_uint(x[k] * c);
+  } else if (kOut == SARR_BF16) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * k] * c, x[2 * k + 1] * c);
+      memcpy(&w[k], &h, 4);
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const __half2 h = __floats2half2_rn(x[2 * k] * c, x[2 * k + 1] * c);
+      memcpy(&w[k], &h, 4);
+    }
+  }
+  reinterpret_cast<uint4*>(o)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+  if (kOut == SARR_F32 && n == 8) reinterpret_cast<uint4*>(o)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+}
+
+template <int kIn, int kOut>
+__device__ __forceinline__ void piece_clip(const Entry& E, int64_t piece, float c) {
+  constexpr int kPer = kIn == SARR_F32 ? 4 : 8, kOutSize = kOut == SARR_F32 ? 4 : 2;
+  constexpr int kElems = kThreads * kVecs * kPer;
+  const int64_t at = piece * kElems, end = E.lead + E.count;
   if (!E.vec) {  // out is aligned otherwise than in: element by element
-    for (int v = threadIdx.x; v < kPiece; v += kThreads) {
+    for (int v = threadIdx.x; v < kElems; v += kThreads) {
       const int64_t i = at + v - E.lead;
-      if (i >= 0 && i < E.count) store_float(E.out, E.out_type, i, load_as_float(E.in, E.type, i) * c);
+      if (i >= 0 && i < E.count) store_float(E.out, kOut, i, load_as_float(E.in, kIn, i) * c);
     }
     return;
   }
-  const int out_size = E.out_type == SARR_F32 ? 4 : 2;
-  const char* base = static_cast<const char*>(E.in) - (int64_t)E.lead * (16 / per);
-  char* obase = static_cast<char*>(E.out) - (int64_t)E.lead * out_size;
-  for (int v = threadIdx.x; v < kPiece / per; v += kThreads) {
-    const int64_t i = at + (int64_t)v * per;
-    if (i >= E.lead && i + per <= end) {
-      const uint4 q = *reinterpret_cast<const uint4*>(base + i * (16 / per));
+  const uint4* p = reinterpret_cast<const uint4*>(static_cast<const char*>(E.in) - E.lead * (16 / kPer)) + at / kPer;
+  char* o = static_cast<char*>(E.out) + (at - E.lead) * kOutSize;
+  const bool whole = at >= E.lead && at + kElems <= end;
+  uint4 q[kVecs];
+#pragma unroll
+  for (int k = 0; k < kVecs; ++k) {
+    const int64_t i = at + (int64_t)(k * kThreads + threadIdx.x) * kPer;
+    if (whole || (i >= E.lead && i + kPer <= end)) q[k] = p[k * kThreads + threadIdx.x];
+  }
+#pragma unroll
+  for (int k = 0; k < kVecs; ++k) {
+    const int v = k * kThreads + threadIdx.x;
+    const int64_t i = at + (int64_t)v * kPer;
+    if (whole || (i >= E.lead && i + kPer <= end)) {
       float x[8];
-      unpack(q, E.type, x);
-      uint32_t w[8];
-      if (E.out_type == SARR_F32) {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) w[k] = __float_as_uint(x[k] * c);
-      } else if (E.out_type == SARR_BF16) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * k] * c, x[2 * k + 1] * c);
-          memcpy(&w[k], &h, 4);
-        }
-      } else {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const __half2 h = __floats2half2_rn(x[2 * k] * c, x[2 * k + 1] * c);
-          memcpy(&w[k], &h, 4);
-        }
-      }
-      uint4* o = reinterpret_cast<uint4*>(obase + i * out_size);
-      o[0] = make_uint4(w[0], w[1], w[2], w[3]);
-      if (out_size == 4 && per == 8) o[1] = make_uint4(w[4], w[5], w[6], w[7]);
+      unpack(q[k], kIn, x);
+      store_scaled<kOut>(o + (int64_t)v * kPer * kOutSize, x, kPer, c);
     } else {
-      for (int k = 0; k < per; ++k) {
-        const int64_t j = i + k - E.lead;
-        if (j >= 0 && j < E.count) store_float(E.out, E.out_type, j, load_as_float(E.in, E.type, j) * c);
+      for (int j = 0; j < kPer; ++j) {
+        const int64_t e = i + j - E.lead;
+        if (e >= 0 && e < E.count) store_float(E.out, kOut, e, load_as_float(E.in, kIn, e) * c);
       }
     }
   }
+}
+
+template <int kIn, int kOut>
+__device__ __forceinline__ void clip_run(const Entry& E, int64_t from, int64_t to, float c) {
+  for (int64_t p = to - 1; p >= from; --p) piece_clip<kIn, kOut>(E, p, c);
 }
 
 template <int kMax, bool kInf>
@@ -275,21 +320,27 @@ __global__ void __launch_bounds__(kThreads) clip_kernel(const __grid_constant__ 
   const double norm = total_norm<kInf>(partial, n_partial);
   if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = (float)norm;
   const float c = clip_coef(norm, max_norm);
-  const int64_t p0 = L.pieces * blockIdx.x / gridDim.x, p1 = L.pieces * (blockIdx.x + 1) / gridDim.x;
+  const int64_t p0 = L.pieces * blockIdx.x / gridDim.x;
+  int64_t p1 = L.pieces * (blockIdx.x + 1) / gridDim.x;
   if (p0 >= p1) return;
-  int t = find_tensor(L, p1 - 1);
-  int64_t first = first_piece(L, t);
-  for (int64_t p = p1 - 1; p >= p0; --p) {
-    while (p < first) first = first_piece(L, --t);
-    // in place and nothing to clip: c x is x
-    if (c == 1.0f && L.e[t].out == L.e[t].in) continue;
-    piece_clip(L.e[t], (p - first) * kPiece, c);
+  for (int t = find_tensor(L, p1 - 1); p1 > p0; --t) {
+    const Entry E = L.e[t];
+    const int64_t first = first_piece(L, t), from = max(p0, first) - first, to = p1 - first;
+    p1 = max(p0, first);
+    if (c == 1.0f && E.out == E.in) continue;  // in place and nothing to clip: c x is x
+    if (E.type == SARR_F32) clip_run<SARR_F32, SARR_F32>(E, from, to, c);
+    else if (E.type == SARR_BF16 && E.out_type == SARR_BF16) clip_run<SARR_BF16, SARR_BF16>(E, from, to, c);
+    else if (E.type == SARR_BF16) clip_run<SARR_BF16, SARR_F32>(E, from, to, c);
+    else if (E.out_type == SARR_F16) clip_run<SARR_F16, SARR_F16>(E, from, to, c);
+    else clip_run<SARR_F16, SARR_F32>(E, from, to, c);
   }
 }
 
 // ---------------------------------------------------------------------------
 // Adam
 // ---------------------------------------------------------------------------
+constexpr int kAdamVecs = 2, kAdamPiece = kThreads * kAdamVecs * 4;  // elements
+
 struct AdamRange {
   int64_t begin, count;  // elements of param / exp_avg / exp_avg_sq
   int64_t grad_begin;
@@ -334,42 +385,50 @@ __global__ void __launch_bounds__(kThreads) adam_kernel(const __grid_constant__ 
   for (int64_t p = p1 - 1; p >= p0; --p) {
     while (t > 0 && p < A.r[t - 1].piece_end) --t;
     const AdamRange& R = A.r[t];
-    const int64_t at = (p - (t > 0 ? A.r[t - 1].piece_end : 0)) * kPiece;
+    const int64_t at = (p - (t > 0 ? A.r[t - 1].piece_end : 0)) * kAdamPiece - R.lead, count = R.count;
     float* P = param + R.begin;
     float* M = exp_avg + R.begin;
     float* V = exp_avg_sq + R.begin;
     const float* G = grad + R.grad_begin;
+    const float step_size = R.step_size;
     if (R.vec) {
-      for (int v = threadIdx.x; v < kPiece / 4; v += kThreads) {
-        const int64_t i = at + 4 * v - R.lead;
-        if (i >= 0 && i + 4 <= R.count) {
-          float4 p4 = *reinterpret_cast<const float4*>(P + i);
-          const float4 g4 = *reinterpret_cast<const float4*>(G + i);
-          float4 m4 = *reinterpret_cast<const float4*>(M + i);
-          float4 v4 = *reinterpret_cast<const float4*>(V + i);
-          p4.x = adam_one(A, R.step_size, p4.x, g4.x * c, m4.x, v4.x);
-          p4.y = adam_one(A, R.step_size, p4.y, g4.y * c, m4.y, v4.y);
-          p4.z = adam_one(A, R.step_size, p4.z, g4.z * c, m4.z, v4.z);
-          p4.w = adam_one(A, R.step_size, p4.w, g4.w * c, m4.w, v4.w);
-          *reinterpret_cast<float4*>(P + i) = p4;
-          *reinterpret_cast<float4*>(M + i) = m4;
-          *reinterpret_cast<float4*>(V + i) = v4;
+      float4 p4[kAdamVecs], g4[kAdamVecs], m4[kAdamVecs], v4[kAdamVecs];
+#pragma unroll
+      for (int k = 0; k < kAdamVecs; ++k) {
+        const int64_t i = at + 4 * (k * kThreads + (int)threadIdx.x);
+        if (i >= 0 && i + 4 <= count) {
+          g4[k] = *reinterpret_cast<const float4*>(G + i);
+          p4[k] = __ldcs(reinterpret_cast<const float4*>(P + i));
+          m4[k] = __ldcs(reinterpret_cast<const float4*>(M + i));
+          v4[k] = __ldcs(reinterpret_cast<const float4*>(V + i));
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < kAdamVecs; ++k) {
+        const int64_t i = at + 4 * (k * kThreads + (int)threadIdx.x);
+        if (i >= 0 && i + 4 <= count) {
+          p4[k].x = adam_one(A, step_size, p4[k].x, g4[k].x * c, m4[k].x, v4[k].x);
+          p4[k].y = adam_one(A, step_size, p4[k].y, g4[k].y * c, m4[k].y, v4[k].y);
+          p4[k].z = adam_one(A, step_size, p4[k].z, g4[k].z * c, m4[k].z, v4[k].z);
+          p4[k].w = adam_one(A, step_size, p4[k].w, g4[k].w * c, m4[k].w, v4[k].w);
+          __stcs(reinterpret_cast<float4*>(P + i), p4[k]);
+          __stcs(reinterpret_cast<float4*>(M + i), m4[k]);
+          __stcs(reinterpret_cast<float4*>(V + i), v4[k]);
         } else {
-          for (int k = 0; k < 4; ++k)
-            if (i + k >= 0 && i + k < R.count) {
-              float m = M[i + k], w = V[i + k];
-              P[i + k] = adam_one(A, R.step_size, P[i + k], G[i + k] * c, m, w);
-              M[i + k] = m;
-              V[i + k] = w;
-            }
+          for (int64_t e = max(i, (int64_t)0); e < min(i + 4, count); ++e) {
+            float m = M[e], w = V[e];
+            P[e] = adam_one(A, step_size, P[e], G[e] * c, m, w);
+            M[e] = m;
+            V[e] = w;
+          }
         }
       }
     } else {
-      for (int v = threadIdx.x; v < kPiece; v += kThreads) {
-        const int64_t i = at + v - R.lead;
-        if (i >= 0 && i < R.count) {
+      for (int v = threadIdx.x; v < kAdamPiece; v += kThreads) {
+        const int64_t i = at + v;
+        if (i >= 0 && i < count) {
           float m = M[i], w = V[i];
-          P[i] = adam_one(A, R.step_size, P[i], G[i] * c, m, w);
+          P[i] = adam_one(A, step_size, P[i], G[i] * c, m, w);
           M[i] = m;
           V[i] = w;
         }
@@ -425,28 +484,31 @@ int check_list(const ListArgs& a) {
 int check_overlap(const ListArgs& a) {
   struct Span {
     uintptr_t begin, end;
-    bool out;
   };
   if (a.n == 0) return SARR_OK;
-  Span* s = new (std::nothrow) Span[2 * (size_t)a.n];
-  if (!s) return SARR_ERR_WORKSPACE;
-  size_t k = 0;
+  Span* out = new (std::nothrow) Span[2 * (size_t)a.n];
+  if (!out) return SARR_ERR_WORKSPACE;
+  Span* in = out + a.n;
+  size_t n_out = 0, n_in = 0;
   for (int i = 0; i < a.n; ++i) {
     if (a.counts[i] == 0) continue;
     const uintptr_t g = reinterpret_cast<uintptr_t>(a.grads[i]), o = reinterpret_cast<uintptr_t>(a.outs[i]);
     const int ot = a.out_types ? a.out_types[i] : a.types[i];
-    s[k++] = Span{o, o + (uintptr_t)a.counts[i] * type_size(ot), true};
-    if (g != o) s[k++] = Span{g, g + (uintptr_t)a.counts[i] * type_size(a.types[i]), false};
+    out[n_out++] = Span{o, o + (uintptr_t)a.counts[i] * type_size(ot)};
+    if (g != o) in[n_in++] = Span{g, g + (uintptr_t)a.counts[i] * type_size(a.types[i])};
   }
-  std::sort(s, s + k, [](const Span& x, const Span& y) { return x.begin < y.begin; });
-  uintptr_t out_end = 0, in_end = 0;
+  const auto before = [](const Span& x, const Span& y) { return x.begin < y.begin; };
+  if (!std::is_sorted(out, out + n_out, before)) std::sort(out, out + n_out, before);
+  if (!std::is_sorted(in, in + n_in, before)) std::sort(in, in + n_in, before);
   bool ok = true;
-  for (size_t i = 0; i < k && ok; ++i) {
-    ok = s[i].begin >= out_end && !(s[i].out && s[i].begin < in_end);
-    uintptr_t& end = s[i].out ? out_end : in_end;
-    end = std::max(end, s[i].end);
+  for (size_t i = 1; i < n_out && ok; ++i) ok = out[i - 1].end <= out[i].begin;
+  // the destinations are disjoint now: each source is held against those that
+  // end behind its begin
+  for (size_t i = 0, j = 0; i < n_in && ok; ++i) {
+    while (j < n_out && out[j].end <= in[i].begin) ++j;
+    ok = j == n_out || out[j].begin >= in[i].end;
   }
-  delete[] s;
+  delete[] out;
   return ok ? SARR_OK : SARR_ERR_ARG;
 }
 
@@ -469,7 +531,8 @@ void fill_list(TensorList<kMax>& L, const ListArgs& a, int begin, int end) {
       E.out_type = (uint8_t)(a.out_types ? a.out_types[i] : a.types[i]);
       E.vec = ((reinterpret_cast<uintptr_t>(E.out) - (uintptr_t)E.lead * type_size(E.out_type)) & 15) == 0;
     }
-    L.pieces += (E.lead + E.count + kPiece - 1) / kPiece;
+    const int64_t piece = kPieceBytes / type_size(E.type);
+    L.pieces += (E.lead + E.count + piece - 1) / piece;
     E.piece_end = L.pieces;
   }
 }
@@ -494,7 +557,7 @@ cudaError_t clip_group(const ListArgs& a, int begin, int end, const double* part
   TensorList<kMax> L;
   fill_list(L, a, begin, end);
   if (L.n == 0) return cudaSuccess;
-  const unsigned ctas = (unsigned)std::min<int64_t>(L.pieces, 148 * 8);
+  const unsigned ctas = (unsigned)std::min<int64_t>(L.pieces, kClipCtas);
   sarr::count_launches(1);
   return sarr::launch(clip_kernel<kMax, kInf>, {dim3(ctas), kThreads, 0, true, 1}, s, L, partial, n_partial,
                       max_norm, norm_out);
@@ -508,8 +571,9 @@ cudaError_t run_list(const ListArgs& a, double max_norm, float* norm_out, double
   bool dependent = false;
   for (int b = 0; b < a.n; b += kLargeList) {
     const int e = std::min(a.n, b + kLargeList), before = n_partial;
-    const cudaError_t st = e - b <= kSmallList
-                               ? norm_group<kSmallList, kInf>(a, b, e, dependent, partial, &n_partial, s)
+    const cudaError_t st =
+        e - b <= kSmallList    ? norm_group<kSmallList, kInf>(a, b, e, dependent, partial, &n_partial, s)
+        : e - b <= kMediumList ? norm_group<kMediumList, kInf>(a, b, e, dependent, partial, &n_partial, s)
                                : norm_group<kLargeList, kInf>(a, b, e, dependent, partial, &n_partial, s);
     if (st != cudaSuccess) return st;
     dependent = dependent || n_partial > before;
@@ -525,8 +589,9 @@ cudaError_t run_list(const ListArgs& a, double max_norm, float* norm_out, double
     bool any = false;
     for (int i = b; i < e; ++i) any = any || a.counts[i] > 0;
     if (!any) continue;
-    const cudaError_t st = e - b <= kSmallList
-                               ? clip_group<kSmallList, kInf>(a, b, e, partial, n_partial, max_norm, out, s)
+    const cudaError_t st =
+        e - b <= kSmallList    ? clip_group<kSmallList, kInf>(a, b, e, partial, n_partial, max_norm, out, s)
+        : e - b <= kMediumList ? clip_group<kMediumList, kInf>(a, b, e, partial, n_partial, max_norm, out, s)
                                : clip_group<kLargeList, kInf>(a, b, e, partial, n_partial, max_norm, out, s);
     if (st != cudaSuccess) return st;
     out = nullptr;
@@ -607,7 +672,7 @@ extern "C" int sarr_adam_step_clipped(int n_ranges, const int64_t* range_begin, 
     R.lead = (uint8_t)lead_of(param + R.begin, 4);
     R.vec = lead_of(grad + R.grad_begin, 4) == R.lead && lead_of(exp_avg + R.begin, 4) == R.lead &&
             lead_of(exp_avg_sq + R.begin, 4) == R.lead;
-    A.pieces += (R.lead + count + kPiece - 1) / kPiece;
+    A.pieces += (R.lead + count + kAdamPiece - 1) / kAdamPiece;
     R.piece_end = A.pieces;
     grads[A.n] = grad + R.grad_begin;
     counts[A.n] = count;
@@ -630,9 +695,9 @@ extern "C" int sarr_adam_step_clipped(int n_ranges, const int64_t* range_begin, 
   if (A.n == 0) return cuda_status(run_list<false>(list, max_norm, norm_out, partial, s));
   int n_partial = 0;
   cudaError_t e = A.n <= kSmallList ? norm_group<kSmallList, false>(list, 0, A.n, false, partial, &n_partial, s)
-                                    : norm_group<kLargeList, false>(list, 0, A.n, false, partial, &n_partial, s);
+                                    : norm_group<kMediumList, false>(list, 0, A.n, false, partial, &n_partial, s);
   if (e != cudaSuccess) return cuda_status(e);
-  const unsigned ctas = (unsigned)std::min<int64_t>(A.pieces, 148 * 8);
+  const unsigned ctas = (unsigned)std::min<int64_t>(A.pieces, kAdamCtas);
   sarr::count_launches(1);
   return cuda_status(sarr::launch(adam_kernel, {dim3(ctas), kThreads, 0, true, 1}, s, A, partial, n_partial,
                                   max_norm, param, grad, exp_avg, exp_avg_sq, norm_out));

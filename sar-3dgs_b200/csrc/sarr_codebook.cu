@@ -159,233 +159,321 @@ __global__ void __launch_bounds__(kLookupThreads) lookup_kernel(const LookupArgs
 // ---------------------------------------------------------------------------
 // sort
 // ---------------------------------------------------------------------------
-// A stable radix sort of the keys (the codes, `codes` for none) from the low
-// digit to the high one. A pass cuts the keys into one contiguous run per CTA
-// and each run into one contiguous part per warp; the place of a key is
-//   keys of smaller digits + the same digit in earlier CTAs + in earlier warps
-//   of the CTA + earlier in the warp's part,
-// the last term from a match over the warp's lanes and a per-warp counter.
+// A stable sort of the keys (the codes, `codes` for none). The unit is a tile of
+// up to 8192 keys that one CTA sorts in registers and shared memory: each warp
+// holds a contiguous part of the tile, 32 keys a round; a key's rank among the
+// warp's keys of its digit is a running count plus the lower lanes that vote for
+// the same digit (one vote per bit, so a digit of 7 bits costs 7 votes whatever
+// the keys are), and one scan over (digit, warp) gives every rank its place.
+//
+// Up to 8192 keys: one CTA, every digit, and the offsets (sort_tile_kernel).
+//
+// More: passes over digits of up to 13 bits (so one pass up to 8191 codes), of
+// three kernels each, which the scheduler may overlap:
+//   histogram  each tile's count of every digit, [tiles][bins]
+//   prefix     per digit the counts of the earlier tiles, and the total
+//   scatter    the tile sorted by the digit, written out behind the smaller digits
+//              and the earlier tiles (in runs, since the tile is in order). The
+//              first pass sorts its tile before it waits for the other two.
+// With one pass the scan over the totals is the offsets.
 constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32;
-constexpr int kMaxDigitBits = 9, kMaxBins = 1 << kMaxDigitBits;
-constexpr int kSortCtas = 148;
-constexpr int kClusterCtas = 8;
-constexpr int kMaxClusterKeys = 65536;  // up to here one cluster sorts in one launch
-constexpr int kBatch = 4;               // rounds of 32 keys loaded together
+constexpr int kTileRounds = 8, kTile = kSortThreads * kTileRounds;
+constexpr int kLocalBits = 7;                          // of a pass inside a tile
+constexpr int kMaxDigitBits = 13, kMaxBins = 1 << kMaxDigitBits;
+constexpr int kCountPitch = kSortWarps + 1;            // [digit][warp], padded against bank conflicts
+constexpr int kCountWords = kCountPitch << kLocalBits;
+constexpr int kPrefixThreads = 256, kPrefixBins = 32;  // bins of a CTA; its threads split the tiles 8 ways
 
 struct SortArgs {
   int n;
   uint32_t codes;
-  int passes, digit_bits, run;  // run: keys of a CTA, a multiple of kSortThreads
   bool wide;
   const void* index;
-  uint32_t* key[2];
-  int32_t* place[2];
-  int32_t* counts;  // [CTAs][bins]
-  int32_t *order, *sorted, *offsets;
-};
-
-struct SortPass {
-  const uint32_t* key_in;    // null: the indexes
+  const uint32_t* key_in;  // null: the indexes
   const int32_t* place_in;
   uint32_t* key_out;
   int32_t* place_out;
-  int shift, bins;
+  int32_t *counts, *totals;  // [tiles][bins], [bins]
+  int shift, bits;           // of this pass's digit
+  int tiles;
+  int32_t* offsets;          // written by the scatter of a sort of one pass, else null
 };
 
-__device__ __forceinline__ SortPass sort_pass(const SortArgs& a, int p) {
-  SortPass P;
-  P.key_in = p == 0 ? nullptr : a.key[(p - 1) & 1];
-  P.place_in = p == 0 ? nullptr : a.place[(p - 1) & 1];
-  const bool last = p == a.passes - 1;
-  P.key_out = last ? reinterpret_cast<uint32_t*>(a.sorted) : a.key[p & 1];
-  P.place_out = last ? a.order : a.place[p & 1];
-  P.shift = p * a.digit_bits;
-  P.bins = 1 << a.digit_bits;
-  return P;
-}
+struct TileShared {
+  uint32_t key[kTile];
+  int32_t place[kTile];
+  int32_t count[kCountWords];
+  int32_t warp_sum[kSortWarps];
+};
 
-__device__ __forceinline__ uint32_t sort_key(const SortArgs& a, const SortPass& P, int i) {
-  return P.key_in ? __ldcg(P.key_in + i) : code_of(a.index, a.wide, i, a.codes);
-}
-
-// Keys of each digit in this warp's part, into hist (the warp's row).
-__device__ __forceinline__ void warp_histogram(const SortArgs& a, const SortPass& P, int begin, int end,
-                                               int32_t* hist) {
-  const int lane = threadIdx.x & 31;
-  for (int d = lane; d < P.bins; d += 32) hist[d] = 0;
-  __syncwarp();
-  for (int i0 = begin; i0 < end; i0 += 32 * kBatch) {
-    uint32_t digit[kBatch];
+// Exclusive scan over the CTA's threads.
+__device__ __forceinline__ int block_scan(int x, int32_t* warp_sum) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int incl = x;
 #pragma unroll
-    for (int k = 0; k < kBatch; ++k) {
-      const int i = i0 + 32 * k + lane;
-      digit[k] = i < end ? (sort_key(a, P, i) >> P.shift) & (P.bins - 1) : (uint32_t)kMaxBins;
-    }
-#pragma unroll
-    for (int k = 0; k < kBatch; ++k) {
-      const uint32_t peers = __match_any_sync(0xffffffffu, digit[k]);
-      if (digit[k] < (uint32_t)kMaxBins && lane == __ffs(peers) - 1) hist[digit[k]] += __popc(peers);
-      __syncwarp();
-    }
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += y;
   }
-}
-
-// One pass's ranges of this CTA and warp.
-__device__ __forceinline__ void sort_range(const SortArgs& a, int cta, int* begin, int* end) {
-  const int part = a.run / kSortWarps, warp = threadIdx.x >> 5;
-  const int64_t b = (int64_t)cta * a.run + (int64_t)warp * part;
-  *begin = (int)(b < a.n ? b : a.n);
-  *end = (int)(b + part < a.n ? b + part : a.n);
-}
-
-// Histograms of this CTA's warps (s_hist [warps][bins]) and their sum, in counts.
-__device__ __forceinline__ void count_phase(const SortArgs& a, const SortPass& P, int cta, int32_t* s_hist) {
-  int begin, end;
-  sort_range(a, cta, &begin, &end);
-  warp_histogram(a, P, begin, end, s_hist + (threadIdx.x >> 5) * P.bins);
+  if (lane == 31) warp_sum[warp] = incl;
   __syncthreads();
-  for (int d = threadIdx.x; d < P.bins; d += kSortThreads) {
-    int sum = 0;
-    for (int w = 0; w < kSortWarps; ++w) sum += s_hist[w * P.bins + d];
-    __stcg(a.counts + (int64_t)cta * P.bins + d, sum);
+  int before = lane < warp ? warp_sum[lane] : 0;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+  __syncthreads();
+  return before + incl - x;
+}
+
+// One stable pass over the tile's keys, which the threads hold: element
+// (warp * rounds + r) * 32 + lane in key[r]. On return S holds the tile in order
+// and so do the threads.
+__device__ __forceinline__ void tile_pass(TileShared& S, uint32_t (&key)[kTileRounds], int32_t (&place)[kTileRounds],
+                                          int rounds, int len, int shift, int bits) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, bins = 1 << bits;
+  for (int i = tid; i < bins * kCountPitch; i += kSortThreads) S.count[i] = 0;
+  __syncthreads();
+  int rank[kTileRounds];
+#pragma unroll
+  for (int r = 0; r < kTileRounds; ++r) {
+    if (r < rounds) {
+      const bool have = (warp * rounds + r) * 32 + lane < len;
+      const uint32_t digit = (key[r] >> shift) & (bins - 1);
+      uint32_t peers = __ballot_sync(0xffffffffu, have);
+#pragma unroll
+      for (int b = 0; b < kLocalBits; ++b) {  // the bits above `bits` are 0 in every lane
+        const bool one = (digit >> b) & 1;
+        const uint32_t ones = __ballot_sync(0xffffffffu, one);
+        peers &= one ? ones : ~ones;
+      }
+      const uint32_t below = peers & ((1u << lane) - 1);
+      int32_t* at = S.count + digit * kCountPitch + warp;
+      const int before = have ? *at : 0;
+      __syncwarp();
+      if (have && below == 0) *at = before + __popc(peers);
+      __syncwarp();
+      rank[r] = before + __popc(below);
+    }
+  }
+  __syncthreads();
+  {  // scan in the order (digit, warp): bins / 32 entries per thread, at least one
+    const int each = bins >= 32 ? bins / 32 : 1, first = tid * each;
+    int x[(1 << kLocalBits) / 32], sum = 0;
+#pragma unroll
+    for (int k = 0; k < (1 << kLocalBits) / 32; ++k) {
+      const int e = first + k;
+      x[k] = k < each && e < bins * 32 ? S.count[(e >> 5) * kCountPitch + (e & 31)] : 0;
+      sum += x[k];
+    }
+    int at = block_scan(sum, S.warp_sum);
+#pragma unroll
+    for (int k = 0; k < (1 << kLocalBits) / 32; ++k) {
+      const int e = first + k;
+      if (k < each && e < bins * 32) S.count[(e >> 5) * kCountPitch + (e & 31)] = at;
+      at += x[k];
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < kTileRounds; ++r) {
+    if (r < rounds && (warp * rounds + r) * 32 + lane < len) {
+      const int to = S.count[((key[r] >> shift) & (bins - 1)) * kCountPitch + warp] + rank[r];
+      S.key[to] = key[r];
+      S.place[to] = place[r];
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < kTileRounds; ++r) {
+    const int e = (warp * rounds + r) * 32 + lane;
+    if (r < rounds && e < len) {
+      key[r] = S.key[e];
+      place[r] = S.place[e];
+    }
   }
 }
 
-// From the counts of all CTAs and this CTA's warp histograms: the place of each
-// warp's first key of each digit (s_hist, in place), then the keys to their
-// places.
-__device__ __forceinline__ void scatter_phase(const SortArgs& a, const SortPass& P, int cta, int ctas,
-                                              int32_t* s_hist, int32_t* s_below, int32_t* s_total) {
+// The tile's keys into the threads, then sorted by `bits` bits from `shift`.
+__device__ __forceinline__ void sort_tile(const SortArgs& a, TileShared& S, uint32_t (&key)[kTileRounds],
+                                          int32_t (&place)[kTileRounds], int tile0, int len, int rounds, int shift,
+                                          int bits) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int r = 0; r < kTileRounds; ++r) {
+    const int e = (warp * rounds + r) * 32 + lane;
+    key[r] = 0;
+    place[r] = 0;
+    if (r < rounds && e < len) {
+      const int i = tile0 + e;
+      key[r] = a.key_in ? __ldcg(a.key_in + i) : code_of(a.index, a.wide, i, a.codes);
+      place[r] = a.key_in ? __ldcg(a.place_in + i) : i;
+    }
+  }
+  const int passes = (bits + kLocalBits - 1) / kLocalBits, each = (bits + passes - 1) / passes;
+  for (int p = 0; p < passes; ++p)
+    tile_pass(S, key, place, rounds, len, shift + p * each, min(each, bits - p * each));
+}
+
+extern __shared__ __align__(16) unsigned char s_sort[];
+
+__global__ void __launch_bounds__(kSortThreads) sort_tile_kernel(const SortArgs a) {
+  TileShared& S = *reinterpret_cast<TileShared*>(s_sort);
+  uint32_t key[kTileRounds];
+  int32_t place[kTileRounds];
+  sarr::dependents_may_start();
+  const int rounds = (a.n + kSortThreads - 1) / kSortThreads;
+  sort_tile(a, S, key, place, 0, a.n, rounds, 0, a.bits);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int r = 0; r < kTileRounds; ++r) {
+    const int e = (warp * rounds + r) * 32 + lane;
+    if (r < rounds && e < a.n) {
+      a.key_out[e] = key[r];
+      a.place_out[e] = place[r];
+    }
+  }
+  // the first place whose key is >= c
+#pragma unroll 4
+  for (int64_t c = threadIdx.x; c <= a.codes; c += kSortThreads) {
+    int lo = 0, hi = a.n;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (S.key[mid] < (uint32_t)c) lo = mid + 1;
+      else hi = mid;
+    }
+    a.offsets[c] = lo;
+  }
+}
+
+__global__ void __launch_bounds__(kSortThreads) sort_histogram_kernel(const SortArgs a) {
+  __shared__ int32_t s_bin[kMaxBins];
+  sarr::dependents_may_start();
+  sarr::wait_for_previous();
+  const int bins = 1 << a.bits, tile0 = blockIdx.x * kTile, len = min(kTile, a.n - tile0);
+  for (int d = threadIdx.x; d < bins; d += kSortThreads) s_bin[d] = 0;
+  uint32_t key[kTileRounds];
+#pragma unroll
+  for (int r = 0; r < kTileRounds; ++r) {
+    const int e = r * kSortThreads + threadIdx.x;
+    if (e < len) key[r] = a.key_in ? __ldcg(a.key_in + tile0 + e) : code_of(a.index, a.wide, tile0 + e, a.codes);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < kTileRounds; ++r)
+    if (r * kSortThreads + threadIdx.x < len) atomicAdd(s_bin + ((key[r] >> a.shift) & (bins - 1)), 1);
+  __syncthreads();
+  for (int d = threadIdx.x; d < bins; d += kSortThreads) a.counts[(int64_t)blockIdx.x * bins + d] = s_bin[d];
+}
+
+// counts[t][d] becomes the sum of counts[0 .. t-1][d], totals[d] the sum of all.
+__global__ void __launch_bounds__(kPrefixThreads) sort_prefix_kernel(const SortArgs a) {
+  constexpr int kSplit = kPrefixThreads / kPrefixBins;
+  __shared__ int32_t s_sum[kSplit][kPrefixBins];
+  sarr::dependents_may_start();
+  sarr::wait_for_previous();
+  const int bins = 1 << a.bits, d = blockIdx.x * kPrefixBins + (threadIdx.x & (kPrefixBins - 1));
+  const int part = threadIdx.x / kPrefixBins, per = (a.tiles + kSplit - 1) / kSplit;
+  const int t0 = min(part * per, a.tiles), t1 = min(t0 + per, a.tiles);
+  int32_t* c = a.counts + d;
+  int sum = 0;
+  if (d < bins) {
+#pragma unroll 16
+    for (int t = t0; t < t1; ++t) sum += __ldcg(c + (int64_t)t * bins);
+  }
+  s_sum[part][threadIdx.x & (kPrefixBins - 1)] = sum;
+  __syncthreads();
+  if (d >= bins) return;
+  int at = 0, all = 0;
+#pragma unroll
+  for (int k = 0; k < kSplit; ++k) {
+    const int x = s_sum[k][threadIdx.x & (kPrefixBins - 1)];
+    if (k < part) at += x;
+    all += x;
+  }
+  if (part == 0) a.totals[d] = all;
+  for (int t = t0; t < t1; t += 16) {
+    int x[16];
+#pragma unroll
+    for (int k = 0; k < 16; ++k) x[k] = t + k < t1 ? __ldcg(c + (int64_t)(t + k) * bins) : 0;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+      if (t + k < t1) c[(int64_t)(t + k) * bins] = at;
+      at += x[k];
+    }
+  }
+}
+
+__global__ void __launch_bounds__(kSortThreads) sort_scatter_kernel(const SortArgs a) {
+  TileShared& S = *reinterpret_cast<TileShared*>(s_sort);
+  int32_t* s_base = reinterpret_cast<int32_t*>(s_sort + sizeof(TileShared));  // [bins]
+  uint32_t key[kTileRounds];
+  int32_t place[kTileRounds];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  // below: the digit's keys in earlier CTAs; total: in all. Several threads per digit.
-  for (int d = tid; d < P.bins; d += kSortThreads) s_below[d] = s_total[d] = 0;
-  __syncthreads();
+  const int bins = 1 << a.bits, tile0 = blockIdx.x * kTile, len = min(kTile, a.n - tile0);
+  const int rounds = (len + kSortThreads - 1) / kSortThreads;
+  sarr::dependents_may_start();
+  if (a.key_in) sarr::wait_for_previous();  // the first pass's keys are the caller's
+  sort_tile(a, S, key, place, tile0, len, rounds, a.shift, a.bits);
+  if (!a.key_in) sarr::wait_for_previous();
+  // where each digit begins, and in it this tile's keys
   {
-    const int d = tid & (P.bins - 1), part = tid / P.bins, parts = kSortThreads / P.bins;
-    int below = 0, total = 0;
-#pragma unroll 8
-    for (int c = part; c < ctas; c += parts) {
-      const int x = __ldcg(a.counts + (int64_t)c * P.bins + d);
-      total += x;
-      if (c < cta) below += x;
+    const int each = max(bins / kSortThreads, 1), first = tid * each;
+    int x[kMaxBins / kSortThreads], sum = 0;
+#pragma unroll
+    for (int k = 0; k < kMaxBins / kSortThreads; ++k) {
+      x[k] = k < each && first + k < bins ? __ldcg(a.totals + first + k) : 0;
+      sum += x[k];
     }
-    if (total) {
-      atomicAdd(s_total + d, total);
-      atomicAdd(s_below + d, below);
+    int before[kMaxBins / kSortThreads];
+#pragma unroll
+    for (int k = 0; k < kMaxBins / kSortThreads; ++k)
+      before[k] = k < each && first + k < bins ? __ldcg(a.counts + (int64_t)blockIdx.x * bins + first + k) : 0;
+    int at = block_scan(sum, S.warp_sum);
+#pragma unroll
+    for (int k = 0; k < kMaxBins / kSortThreads; ++k) {
+      const int d = first + k;
+      if (k < each && d < bins) {
+        s_base[d] = at + before[k];
+        if (a.offsets && blockIdx.x == 0 && d <= (int)a.codes) a.offsets[d] = at;
+      }
+      at += x[k];
     }
   }
   __syncthreads();
-  // exclusive scan of the totals by one warp
-  if (warp == 0) {
-    int carry = 0;
-    for (int d0 = 0; d0 < P.bins; d0 += 32) {
-      const int x = d0 + lane < P.bins ? s_total[d0 + lane] : 0;
-      int incl = x;
+  // less the place in the tile where the digit begins
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += y;
-      }
-      if (d0 + lane < P.bins) s_below[d0 + lane] += carry + incl - x;
-      carry += __shfl_sync(0xffffffffu, incl, 31);
+  for (int r = 0; r < kTileRounds; ++r) {
+    const int e = (warp * rounds + r) * 32 + lane;
+    if (r < rounds && e < len) {
+      const uint32_t d = (key[r] >> a.shift) & (bins - 1);
+      if (e == 0 || ((S.key[e - 1] >> a.shift) & (bins - 1)) != d) s_base[d] -= e;
     }
   }
   __syncthreads();
-  for (int d = tid; d < P.bins; d += kSortThreads) {
-    int at = s_below[d];
-    for (int w = 0; w < kSortWarps; ++w) {
-      const int x = s_hist[w * P.bins + d];
-      s_hist[w * P.bins + d] = at;
-      at += x;
-    }
-  }
-  __syncthreads();
-  int begin, end;
-  sort_range(a, cta, &begin, &end);
-  int32_t* next = s_hist + warp * P.bins;
-  for (int i0 = begin; i0 < end; i0 += 32 * kBatch) {
-    uint32_t key[kBatch];
-    int32_t place[kBatch];
 #pragma unroll
-    for (int k = 0; k < kBatch; ++k) {
-      const int i = i0 + 32 * k + lane;
-      key[k] = i < end ? sort_key(a, P, i) : 0u;
-      place[k] = i < end ? (P.place_in ? __ldcg(P.place_in + i) : i) : 0;
-    }
-#pragma unroll
-    for (int k = 0; k < kBatch; ++k) {
-      const bool have = i0 + 32 * k + lane < end;
-      const uint32_t digit = have ? (key[k] >> P.shift) & (P.bins - 1) : (uint32_t)kMaxBins;
-      const uint32_t peers = __match_any_sync(0xffffffffu, digit);
-      const int leader = __ffs(peers) - 1;
-      int base = 0;
-      if (have && lane == leader) {
-        base = next[digit];
-        next[digit] = base + __popc(peers);
-      }
-      base = __shfl_sync(0xffffffffu, base, leader);
-      __syncwarp();
-      if (have) {
-        const int to = base + __popc(peers & ((1u << lane) - 1));
-        __stcg(P.key_out + to, key[k]);
-        __stcg(P.place_out + to, place[k]);
-      }
+  for (int r = 0; r < kTileRounds; ++r) {
+    const int e = (warp * rounds + r) * 32 + lane;
+    if (r < rounds && e < len) {
+      const int to = s_base[(key[r] >> a.shift) & (bins - 1)] + e;
+      a.key_out[to] = key[r];
+      a.place_out[to] = place[r];
     }
   }
 }
 
-// The first place whose code is >= c.
-__device__ __forceinline__ int lower_bound(const int32_t* sorted, int n, uint32_t c) {
+// The first place whose code is >= c, for each c.
+__global__ void __launch_bounds__(256) sort_offsets_kernel(int n, uint32_t codes, const int32_t* sorted,
+                                                           int32_t* offsets) {
+  sarr::dependents_may_start();
+  sarr::wait_for_previous();
+  const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (c > codes) return;
   int lo = 0, hi = n;
   while (lo < hi) {
     const int mid = lo + (hi - lo) / 2;
-    if ((uint32_t)__ldcg(sorted + mid) < c) lo = mid + 1;
+    if ((uint32_t)sorted[mid] < (uint32_t)c) lo = mid + 1;
     else hi = mid;
   }
-  return lo;
-}
-
-__device__ __forceinline__ void cluster_barrier() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-
-extern __shared__ int32_t s_sort[];  // [warps][bins], then 2 x [bins]
-
-// The whole sort by the CTAs of one cluster.
-__global__ void __launch_bounds__(kSortThreads) sort_cluster_kernel(const SortArgs a) {
-  const int bins = 1 << a.digit_bits, ctas = gridDim.x, cta = blockIdx.x;
-  for (int p = 0; p < a.passes; ++p) {
-    const SortPass P = sort_pass(a, p);
-    count_phase(a, P, cta, s_sort);
-    cluster_barrier();
-    scatter_phase(a, P, cta, ctas, s_sort, s_sort + kSortWarps * bins, s_sort + (kSortWarps + 1) * bins);
-    cluster_barrier();
-  }
-  for (int64_t c = (int64_t)cta * kSortThreads + threadIdx.x; c <= a.codes; c += (int64_t)ctas * kSortThreads)
-    a.offsets[c] = lower_bound(a.sorted, a.n, (uint32_t)c);
-}
-
-__global__ void __launch_bounds__(kSortThreads) sort_count_kernel(const SortArgs a, int p) {
-  sarr::dependents_may_start();
-  sarr::wait_for_previous();
-  count_phase(a, sort_pass(a, p), blockIdx.x, s_sort);
-}
-
-__global__ void __launch_bounds__(kSortThreads) sort_scatter_kernel(const SortArgs a, int p) {
-  sarr::dependents_may_start();
-  sarr::wait_for_previous();
-  const SortPass P = sort_pass(a, p);
-  int begin, end;
-  sort_range(a, blockIdx.x, &begin, &end);
-  warp_histogram(a, P, begin, end, s_sort + (threadIdx.x >> 5) * P.bins);
-  scatter_phase(a, P, blockIdx.x, gridDim.x, s_sort, s_sort + kSortWarps * P.bins,
-                s_sort + (kSortWarps + 1) * P.bins);
-}
-
-__global__ void __launch_bounds__(256) sort_offsets_kernel(const SortArgs a) {
-  sarr::wait_for_previous();
-  const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (c <= a.codes) a.offsets[c] = lower_bound(a.sorted, a.n, (uint32_t)c);
+  offsets[c] = lo;
 }
 
 // ---------------------------------------------------------------------------
@@ -620,7 +708,7 @@ int cuda_status(cudaError_t e) {
 }
 
 constexpr int64_t kMaxCols = 1 << 22;
-constexpr int64_t kMaxCount = 2147483647 - 2 * kSortThreads * kSortCtas;  // Gaussians and codes
+constexpr int64_t kMaxCount = 2147483647 - (1 << 19);  // Gaussians and codes
 
 size_t round256(size_t b) { return (b + 255) & ~(size_t)255; }
 int type_size(int type) { return type == SARR_F32 ? 4 : 2; }
@@ -657,29 +745,32 @@ cudaError_t launch_lookup(LookupArgs a, int v, cudaStream_t s) {
 }
 
 struct SortPlan {
-  int passes, digit_bits, ctas, run;
-  bool cluster;
-  size_t key_bytes, counts_at, bytes;
+  int bits, passes, digit_bits, tiles;
+  size_t key_bytes, counts_at, totals_at, bytes;
 };
 
 SortPlan sort_plan(int64_t n, int64_t codes) {
   SortPlan P;
-  int bits = 1;
-  while (((int64_t)1 << bits) <= codes) ++bits;  // keys 0 .. codes
-  P.passes = (bits + kMaxDigitBits - 1) / kMaxDigitBits;
-  P.digit_bits = (bits + P.passes - 1) / P.passes;
-  P.cluster = n <= kMaxClusterKeys;
-  P.ctas = P.cluster ? pow2_at_least((n + 4095) / 4096, kClusterCtas) : kSortCtas;
-  P.run = (int)(((n + P.ctas - 1) / P.ctas + kSortThreads - 1) / kSortThreads * kSortThreads);
-  P.key_bytes = round256((size_t)n * 4);
-  const int buffers = std::min(P.passes - 1, 2);
-  P.counts_at = (size_t)buffers * 2 * P.key_bytes;
-  P.bytes = P.counts_at + round256((size_t)P.ctas * (4u << P.digit_bits)) + 256;
+  P.bits = 1;
+  while (((int64_t)1 << P.bits) <= codes) ++P.bits;  // keys 0 .. codes
+  P.passes = (P.bits + kMaxDigitBits - 1) / kMaxDigitBits;
+  P.digit_bits = (P.bits + P.passes - 1) / P.passes;
+  P.tiles = (int)((n + kTile - 1) / kTile);
+  P.key_bytes = P.counts_at = P.totals_at = 0;
+  P.bytes = 0;  // one tile: shared memory holds it all
+  if (P.tiles > 1) {
+    P.key_bytes = round256((size_t)n * 4);
+    const int buffers = std::min(P.passes - 1, 2);
+    P.counts_at = (size_t)buffers * 2 * P.key_bytes;
+    P.totals_at = P.counts_at + round256((size_t)P.tiles * (4u << P.digit_bits));
+    P.bytes = P.totals_at + round256(4u << P.digit_bits);
+  }
   return P;
 }
 
-// The sort kernels use more than 48 KB of shared memory; the permission is per
+// The tile kernels use more than 48 KB of shared memory; the permission is per
 // device, asked for once.
+constexpr size_t kTileSmem = sizeof(TileShared);
 cudaError_t allow_sort_smem() {
   static std::atomic<uint64_t> done{0};
   int dev = 0;
@@ -687,15 +778,54 @@ cudaError_t allow_sort_smem() {
   if (e != cudaSuccess) return e;
   const uint64_t bit = dev < 64 ? (uint64_t)1 << dev : 0;
   if (bit & done.load(std::memory_order_acquire)) return cudaSuccess;
-  const int bytes = (kSortWarps + 2) * kMaxBins * 4;
-  const void* kernels[] = {(const void*)sort_cluster_kernel, (const void*)sort_count_kernel,
-                           (const void*)sort_scatter_kernel};
-  for (const void* k : kernels) {
-    e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e != cudaSuccess) return e;
-  }
+  e = cudaFuncSetAttribute(sort_tile_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kTileSmem);
+  if (e != cudaSuccess) return e;
+  e = cudaFuncSetAttribute(sort_scatter_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           (int)(kTileSmem + 4 * kMaxBins));
+  if (e != cudaSuccess) return e;
   done.fetch_or(bit, std::memory_order_release);
   return cudaSuccess;
+}
+
+cudaError_t run_sort(SortArgs a, const SortPlan& P, char* w, int32_t* order, int32_t* sorted, int32_t* offsets,
+                     cudaStream_t s) {
+  if (P.tiles <= 1) {
+    a.key_out = reinterpret_cast<uint32_t*>(sorted);
+    a.place_out = order;
+    a.offsets = offsets;
+    a.bits = P.bits;
+    sarr::count_launches(1);
+    return sarr::launch(sort_tile_kernel, {dim3(1), kSortThreads, kTileSmem, false, 1}, s, a);
+  }
+  a.tiles = P.tiles;
+  a.counts = reinterpret_cast<int32_t*>(w + P.counts_at);
+  a.totals = reinterpret_cast<int32_t*>(w + P.totals_at);
+  cudaError_t e;
+  for (int p = 0; p < P.passes; ++p) {
+    const bool last = p == P.passes - 1;
+    uint32_t* key = last ? reinterpret_cast<uint32_t*>(sorted)
+                         : reinterpret_cast<uint32_t*>(w + (size_t)(2 * (p & 1)) * P.key_bytes);
+    int32_t* place = last ? order : reinterpret_cast<int32_t*>(w + (size_t)(2 * (p & 1) + 1) * P.key_bytes);
+    a.shift = p * P.digit_bits;
+    a.bits = std::min(P.digit_bits, P.bits - a.shift);
+    a.key_out = key;
+    a.place_out = place;
+    a.offsets = P.passes == 1 ? offsets : nullptr;
+    const unsigned bins = 1u << a.bits;
+    sarr::count_launches(3);
+    e = sarr::launch(sort_histogram_kernel, {dim3((unsigned)P.tiles), kSortThreads, 0, p > 0, 1}, s, a);
+    if (e != cudaSuccess) return e;
+    e = sarr::launch(sort_prefix_kernel, {dim3((bins + kPrefixBins - 1) / kPrefixBins), kPrefixThreads, 0, true, 1}, s, a);
+    if (e != cudaSuccess) return e;
+    e = sarr::launch(sort_scatter_kernel, {dim3((unsigned)P.tiles), kSortThreads, kTileSmem + 4 * bins, true, 1}, s, a);
+    if (e != cudaSuccess) return e;
+    a.key_in = key;
+    a.place_in = place;
+  }
+  if (P.passes == 1) return cudaSuccess;
+  sarr::count_launches(1);
+  return sarr::launch(sort_offsets_kernel, {dim3((unsigned)(((int64_t)a.codes + 256) / 256)), 256, 0, true, 1}, s, a.n,
+                      a.codes, sorted, offsets);
 }
 
 struct GradPlan {
@@ -720,6 +850,19 @@ GradPlan grad_plan(int64_t n, int64_t cols, int64_t vecs) {
   P.spans = (n + P.span - 1) / P.span;
   P.bytes = round256((size_t)P.spans * 2 * (size_t)cols * 4) + 256;
   return P;
+}
+
+// What the two gradient entry points check alike.
+int check_gradient(int64_t n, int64_t codes, int64_t cols, const void* grad_rows, int rows_type, int64_t rows_stride,
+                   const void* grad_table, int table_type, int64_t table_stride) {
+  if (n < 0 || n > kMaxCount || codes < 0 || codes > kMaxCount || cols < 0 || cols > kMaxCols) return SARR_ERR_ARG;
+  if (!type_ok(rows_type) || !type_ok(table_type)) return SARR_ERR_ARG;
+  if (rows_type != SARR_F32 && table_type != SARR_F32 && table_type != rows_type) return SARR_ERR_ARG;
+  if (rows_stride < cols || table_stride < cols) return SARR_ERR_ARG;
+  if (codes == 0 || cols == 0) return SARR_OK;
+  if (!grad_table || (n > 0 && !grad_rows)) return SARR_ERR_ARG;
+  if (!aligned(grad_rows, type_size(rows_type)) || !aligned(grad_table, type_size(table_type))) return SARR_ERR_ARG;
+  return SARR_OK;
 }
 
 template <typename TG, typename TT, int kV>
@@ -798,44 +941,17 @@ extern "C" int sarr_codebook_sort(int64_t n, int64_t codes, const void* index, i
   if (!offsets || (n > 0 && (!index || !order || !sorted_codes))) return SARR_ERR_ARG;
   if (!aligned(index, index_bits / 8) || !aligned(order, 4) || !aligned(sorted_codes, 4) || !aligned(offsets, 4))
     return SARR_ERR_ARG;
-  if (!ws || ws_bytes < need || !aligned(ws, 256)) return SARR_ERR_WORKSPACE;
+  if (ws_bytes < need || (need > 0 && (!ws || !aligned(ws, 256)))) return SARR_ERR_WORKSPACE;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   cudaError_t e = allow_sort_smem();
   if (e != cudaSuccess) return cuda_status(e);
-  const SortPlan P = sort_plan(n, codes);
   SortArgs a;
   memset(&a, 0, sizeof(a));
   a.n = (int)n;
   a.codes = (uint32_t)codes;
-  a.passes = P.passes;
-  a.digit_bits = P.digit_bits;
-  a.run = P.run;
   a.wide = index_bits == 64;
   a.index = index;
-  char* w = static_cast<char*>(ws);
-  for (int k = 0; k < 2; ++k) {
-    a.key[k] = reinterpret_cast<uint32_t*>(w + (size_t)2 * k * P.key_bytes);
-    a.place[k] = reinterpret_cast<int32_t*>(w + ((size_t)2 * k + 1) * P.key_bytes);
-  }
-  a.counts = reinterpret_cast<int32_t*>(w + P.counts_at);
-  a.order = order;
-  a.sorted = sorted_codes;
-  a.offsets = offsets;
-  const size_t smem = (size_t)(kSortWarps + 2) * (4u << P.digit_bits);
-  if (P.cluster) {
-    sarr::count_launches(1);
-    return cuda_status(sarr::launch(sort_cluster_kernel,
-                                    {dim3((unsigned)P.ctas), kSortThreads, smem, false, (unsigned)P.ctas}, s, a));
-  }
-  for (int p = 0; p < P.passes; ++p) {
-    sarr::count_launches(2);
-    e = sarr::launch(sort_count_kernel, {dim3((unsigned)P.ctas), kSortThreads, smem, p > 0, 1}, s, a, p);
-    if (e != cudaSuccess) return cuda_status(e);
-    e = sarr::launch(sort_scatter_kernel, {dim3((unsigned)P.ctas), kSortThreads, smem, true, 1}, s, a, p);
-    if (e != cudaSuccess) return cuda_status(e);
-  }
-  sarr::count_launches(1);
-  return cuda_status(sarr::launch(sort_offsets_kernel, {dim3((unsigned)((codes + 256) / 256)), 256, 0, true, 1}, s, a));
+  return cuda_status(run_sort(a, sort_plan(n, codes), static_cast<char*>(ws), order, sorted_codes, offsets, s));
 }
 
 extern "C" int sarr_codebook_grad_workspace_size(int64_t n, int64_t cols, size_t* bytes) {
@@ -853,16 +969,12 @@ extern "C" int sarr_codebook_grad(int64_t n, int64_t codes, int64_t cols, const 
                                   const int32_t* offsets, float scale, void* grad_table, int table_type,
                                   int64_t table_stride, void* ws, size_t ws_bytes, sarr_stream_t stream) {
   size_t need = 0;
-  if (sarr_codebook_grad_workspace_size(n, cols, &need) != SARR_OK || codes < 0 || codes > kMaxCount)
-    return SARR_ERR_ARG;
-  if (!type_ok(rows_type) || !type_ok(table_type)) return SARR_ERR_ARG;
-  if (rows_type != SARR_F32 && table_type != SARR_F32 && table_type != rows_type) return SARR_ERR_ARG;
-  if (rows_stride < cols || table_stride < cols) return SARR_ERR_ARG;
+  const int st = check_gradient(n, codes, cols, grad_rows, rows_type, rows_stride, grad_table, table_type, table_stride);
+  if (st != SARR_OK) return st;
+  if (sarr_codebook_grad_workspace_size(n, cols, &need) != SARR_OK) return SARR_ERR_ARG;
   if (codes == 0 || cols == 0) return SARR_OK;
-  if (!offsets || !grad_table || (n > 0 && (!grad_rows || !order || !sorted_codes))) return SARR_ERR_ARG;
-  if (!aligned(grad_rows, type_size(rows_type)) || !aligned(grad_table, type_size(table_type)) ||
-      !aligned(order, 4) || !aligned(sorted_codes, 4) || !aligned(offsets, 4))
-    return SARR_ERR_ARG;
+  if (!offsets || (n > 0 && (!order || !sorted_codes))) return SARR_ERR_ARG;
+  if (!aligned(order, 4) || !aligned(sorted_codes, 4) || !aligned(offsets, 4)) return SARR_ERR_ARG;
   if (!ws || ws_bytes < need || !aligned(ws, 256)) return SARR_ERR_WORKSPACE;
   const int v = vector_of(cols, grad_rows, type_size(rows_type), rows_stride, grad_table, type_size(table_type),
                           table_stride);
@@ -896,4 +1008,38 @@ extern "C" int sarr_codebook_grad(int64_t n, int64_t codes, int64_t cols, const 
   else
     e = table_type == SARR_F32 ? launch_grad<__half, float>(a, P, v, s) : launch_grad<__half, __half>(a, P, v, s);
   return cuda_status(e);
+}
+
+extern "C" int sarr_codebook_gradient_workspace_size(int64_t n, int64_t codes, int64_t cols, size_t* bytes) {
+  size_t sort = 0, grad = 0;
+  if (!bytes || sarr_codebook_sort_workspace_size(n, codes, &sort) != SARR_OK ||
+      sarr_codebook_grad_workspace_size(n, cols, &grad) != SARR_OK)
+    return SARR_ERR_ARG;
+  // the order, the sorted codes and the offsets, then the two parts' own
+  // workspaces, which are not needed at the same time
+  *bytes = 2 * round256((size_t)n * 4) + round256((size_t)(codes + 1) * 4) + std::max(round256(sort), grad);
+  return SARR_OK;
+}
+
+extern "C" int sarr_codebook_gradient(int64_t n, int64_t codes, int64_t cols, const void* grad_rows, int rows_type,
+                                      int64_t rows_stride, const void* index, int index_bits, float scale,
+                                      void* grad_table, int table_type, int64_t table_stride, void* ws,
+                                      size_t ws_bytes, sarr_stream_t stream) {
+  size_t need = 0;
+  if (sarr_codebook_gradient_workspace_size(n, codes, cols, &need) != SARR_OK) return SARR_ERR_ARG;
+  int st = check_gradient(n, codes, cols, grad_rows, rows_type, rows_stride, grad_table, table_type, table_stride);
+  if (st != SARR_OK) return st;
+  if ((index_bits != 32 && index_bits != 64) || (n > 0 && !index) || !aligned(index, index_bits / 8)) return SARR_ERR_ARG;
+  if (codes == 0 || cols == 0) return SARR_OK;
+  if (!ws || ws_bytes < need || !aligned(ws, 256)) return SARR_ERR_WORKSPACE;
+  char* w = static_cast<char*>(ws);
+  int32_t* order = reinterpret_cast<int32_t*>(w);
+  int32_t* sorted = reinterpret_cast<int32_t*>(w + round256((size_t)n * 4));
+  int32_t* offsets = reinterpret_cast<int32_t*>(w + 2 * round256((size_t)n * 4));
+  char* rest = w + 2 * round256((size_t)n * 4) + round256((size_t)(codes + 1) * 4);
+  const size_t rest_bytes = ws_bytes - (size_t)(rest - w);
+  st = sarr_codebook_sort(n, codes, index, index_bits, order, sorted, offsets, rest, rest_bytes, stream);
+  if (st != SARR_OK) return st;
+  return sarr_codebook_grad(n, codes, cols, grad_rows, rows_type, rows_stride, order, sorted, offsets, scale, grad_table,
+                            table_type, table_stride, rest, rest_bytes, stream);
 }

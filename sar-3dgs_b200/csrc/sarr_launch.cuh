@@ -33,6 +33,10 @@ struct LaunchShape {
 template <typename... KArgs, typename... Args>
 cudaError_t launch(void (*kernel)(KArgs...), const LaunchShape& shape, cudaStream_t stream,
                    Args&&... args) {
+  if (!shape.dependent && shape.cluster <= 1) {  // costs the host less than a launch with attributes
+    kernel<<<shape.grid, shape.threads, shape.smem, stream>>>(static_cast<KArgs>(args)...);
+    return cudaGetLastError();
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = shape.grid;
   cfg.blockDim = dim3(shape.threads);

@@ -5,6 +5,7 @@ the current CUDA stream and caching-allocator workspaces to the C ABI. It has
 no CPU path: a missing library, a CPU tensor or a non-float32 tensor raises.
 ctypes releases the GIL for the duration of each C call.
 """
+import contextlib
 import ctypes
 import os
 import threading
@@ -97,12 +98,15 @@ def _declare(L):
     L.sarr_codebook_sort.argtypes = [I64, I64, P, I, P, P, P, P, SZ, P]
     L.sarr_codebook_grad_workspace_size.argtypes = [I64, I64, SZP]
     L.sarr_codebook_grad.argtypes = [I64, I64, I64, P, I, I64, P, P, P, F, P, I, I64, P, SZ, P]
+    L.sarr_codebook_gradient_workspace_size.argtypes = [I64, I64, I64, SZP]
+    L.sarr_codebook_gradient.argtypes = [I64, I64, I64, P, I, I64, P, I, F, P, I, I64, P, SZ, P]
     L.sarr_grad_norm_workspace_size.argtypes = [I, SZP]
     L.sarr_grad_norm.argtypes = [I, P, P, P, I, P, P, SZ, P]
     L.sarr_clip_grads.argtypes = [I, P, P, P, P, P, I, D, P, P, SZ, P]
     L.sarr_adam_step_clipped.argtypes = [I, P, P, P, P, P, P, P, P, D, D, D, I64, D, P, P, SZ, P]
     for name in ("sarr_codebook_lookup", "sarr_codebook_sort_workspace_size", "sarr_codebook_sort",
                  "sarr_codebook_grad_workspace_size", "sarr_codebook_grad",
+                 "sarr_codebook_gradient_workspace_size", "sarr_codebook_gradient",
                  "sarr_grad_norm_workspace_size", "sarr_grad_norm", "sarr_clip_grads",
                  "sarr_adam_step_clipped", "sarr_workspace_size", "sarr_state_size", "sarr_forward", "sarr_backward",
                  "sarr_backward_scatter",
@@ -148,6 +152,20 @@ def _ptr(t):
 
 def _stream(device):
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+_NO_SWITCH = contextlib.nullcontext()
+
+
+def _on(device):
+    """Context in which `device` is current (nothing to do where it is already)."""
+    return _NO_SWITCH if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+def _raw_stream(device):
+    """PyTorch's current stream of `device` as an address, without a Stream object
+    (which costs more on the host than a small kernel takes)."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def _as_cuda_f32(t, name):

@@ -12,6 +12,7 @@ in 64 bits and returned as a float32 scalar on the device (no synchronisation).
 Results are bitwise reproducible. The reference trains without clipping.
 """
 import ctypes
+import functools
 import math
 from array import array
 from typing import Iterable, Optional, Sequence
@@ -40,23 +41,31 @@ def _dense(t):
 
 
 def _list(tensors, name):
-    """(pointers, counts, types, device) of dense CUDA tensors."""
+    """(pointers, counts, types, device, whether all are contiguous) of dense CUDA tensors."""
+    try:
+        types = [_TYPES[t.dtype] for t in tensors]
+        dev = tensors[0].device
+        contiguous = all([t.is_contiguous() for t in tensors])
+        if (dev.type == "cuda" and [t.get_device() for t in tensors].count(dev.index) == len(tensors)
+                and (contiguous or all([_dense(t) for t in tensors]))):
+            return (array("Q", [t.data_ptr() for t in tensors]), array("q", [t.numel() for t in tensors]),
+                    array("i", types), dev, contiguous)
+    except (AttributeError, KeyError):
+        pass
     dev = None
-    for k, t in enumerate(tensors):
+    for k, t in enumerate(tensors):  # find out which
         if not isinstance(t, torch.Tensor):
             raise TypeError(f"{name}[{k}] must be a torch.Tensor")
         if t.dtype not in _TYPES:
             raise RuntimeError(f"{name}[{k}] must be float32, bfloat16 or float16, got {t.dtype}")
-        if t.device != dev:
-            if not t.is_cuda:
-                raise RuntimeError(f"{name}[{k}] must be a CUDA tensor (there is no CPU path)")
-            if dev is not None:
-                raise RuntimeError(f"{name}[{k}] is on {t.device}, {name}[0] on {dev}")
-            dev = t.device
+        if not t.is_cuda:
+            raise RuntimeError(f"{name}[{k}] must be a CUDA tensor (there is no CPU path)")
+        if dev is not None and t.device != dev:
+            raise RuntimeError(f"{name}[{k}] is on {t.device}, {name}[0] on {dev}")
+        dev = t.device
         if not _dense(t):
             raise RuntimeError(f"{name}[{k}] must be dense, got shape {tuple(t.shape)} with strides {t.stride()}")
-    return (array("Q", [t.data_ptr() for t in tensors]), array("q", [t.numel() for t in tensors]),
-            array("i", [_TYPES[t.dtype] for t in tensors]), dev)
+    raise RuntimeError(f"{name} cannot be used")
 
 
 def _at(a):
@@ -70,17 +79,15 @@ def _norm_kind(norm_type):
     return kind
 
 
-_ws_size = {}
+@functools.lru_cache(maxsize=256)
+def _ws_size(n):
+    out = ctypes.c_size_t()
+    _native._check(_native.lib().sarr_grad_norm_workspace_size(n, ctypes.byref(out)), "sarr_grad_norm_workspace_size")
+    return out.value
 
 
 def _workspace(n, dev):
-    size = _ws_size.get(n)
-    if size is None:
-        out = ctypes.c_size_t()
-        _native._check(_native.lib().sarr_grad_norm_workspace_size(n, ctypes.byref(out)),
-                       "sarr_grad_norm_workspace_size")
-        size = _ws_size[n] = out.value
-    return torch.empty(size, dtype=torch.uint8, device=dev)
+    return torch.empty(_ws_size(n), dtype=torch.uint8, device=dev)
 
 
 def grad_norm(grads: Sequence[torch.Tensor], norm_type: float = 2.0) -> torch.Tensor:
@@ -90,21 +97,21 @@ def grad_norm(grads: Sequence[torch.Tensor], norm_type: float = 2.0) -> torch.Te
     kind = _norm_kind(norm_type)
     if not grads:
         return torch.zeros(())
-    ptrs, counts, types, dev = _list(grads, "grads")
-    with torch.cuda.device(dev):
+    ptrs, counts, types, dev, _ = _list(grads, "grads")
+    with _native._on(dev):
         ws = _workspace(len(grads), dev)
         norm = torch.empty((), dtype=torch.float32, device=dev)
         _native._check(_native.lib().sarr_grad_norm(
             len(grads), _at(ptrs), _at(counts), _at(types), kind, norm.data_ptr(), ws.data_ptr(),
-            ws.numel(), _native._stream(dev)), "sarr_grad_norm")
+            ws.numel(), _native._raw_stream(dev)), "sarr_grad_norm")
     return norm
 
 
 def clip_grads(grads: Sequence[torch.Tensor], max_norm: float, norm_type: float = 2.0,
                out: Optional[Sequence[torch.Tensor]] = None) -> torch.Tensor:
     """Multiplies `grads` by min(1, max_norm / (norm + 1e-6)), in place or into
-    the tensors of `out` (of the gradients' shapes and strides; each of its
-    gradient's type or float32), and returns the norm before clipping. No two
+    the tensors of `out` (as many elements each, contiguous as the gradients are
+    or of their shapes and strides; each of its gradient's type or float32), and returns the norm before clipping. No two
     destinations may overlap, nor a destination another tensor's gradient."""
     grads = list(grads)
     kind = _norm_kind(norm_type)
@@ -116,23 +123,26 @@ def clip_grads(grads: Sequence[torch.Tensor], max_norm: float, norm_type: float 
             raise RuntimeError(f"{len(grads)} gradients and {len(out)} destinations")
     if not grads:
         return torch.zeros(())
-    ptrs, counts, types, dev = _list(grads, "grads")
+    ptrs, counts, types, dev, flat = _list(grads, "grads")
     optrs, otypes = ptrs, types
     if out is not None:
-        optrs, ocounts, otypes, odev = _list(out, "out")
+        optrs, ocounts, otypes, odev, oflat = _list(out, "out")
         if ocounts != counts or odev != dev:
-            raise RuntimeError("out must have the gradients' shapes and device")
-        for k, (g, o) in enumerate(zip(grads, out)):
-            if o.dtype != g.dtype and o.dtype != torch.float32:
-                raise RuntimeError(f"out[{k}] must be {g.dtype} or float32, got {o.dtype}")
-            if o.shape != g.shape or (o.stride() != g.stride() and not (o.is_contiguous() and g.is_contiguous())):
-                raise RuntimeError(f"out[{k}] must have its gradient's shape and strides")
-    with torch.cuda.device(dev):
+            raise RuntimeError("out must have the gradients' sizes and device")
+        if otypes != types:
+            for k, (g, o) in enumerate(zip(grads, out)):
+                if o.dtype != g.dtype and o.dtype != torch.float32:
+                    raise RuntimeError(f"out[{k}] must be {g.dtype} or float32, got {o.dtype}")
+        if not (flat and oflat):
+            for k, (g, o) in enumerate(zip(grads, out)):
+                if o.shape != g.shape or o.stride() != g.stride():
+                    raise RuntimeError(f"out[{k}] must have its gradient's shape and strides")
+    with _native._on(dev):
         ws = _workspace(len(grads), dev)
         norm = torch.empty((), dtype=torch.float32, device=dev)
         _native._check(_native.lib().sarr_clip_grads(
             len(grads), _at(ptrs), _at(counts), _at(types), _at(optrs), _at(otypes), kind,
-            float(max_norm), norm.data_ptr(), ws.data_ptr(), ws.numel(), _native._stream(dev)),
+            float(max_norm), norm.data_ptr(), ws.data_ptr(), ws.numel(), _native._raw_stream(dev)),
             "sarr_clip_grads")
     return norm
 
@@ -171,7 +181,7 @@ def adam_step_clipped(param, grad, exp_avg, exp_avg_sq, segments, step, max_norm
         raise RuntimeError(f"segments must be 1 to {MAX_RANGES} ascending ends, the last one the buffers' {count}")
     if not float(max_norm) >= 0.0:
         raise RuntimeError(f"max_norm must be >= 0, got {max_norm}")
-    with torch.cuda.device(dev):
+    with _native._on(dev):
         ws = _workspace(MAX_RANGES, dev)
         norm = torch.empty((), dtype=torch.float32, device=dev)
         adam_ranges_clipped(tensors, list(zip(begins, ends, begins, [lr for _, lr in segments])), step, max_norm,
@@ -190,4 +200,4 @@ def adam_ranges_clipped(tensors, ranges, step, max_norm, betas, eps, norm, ws):
     _native._check(_native.lib().sarr_adam_step_clipped(
         len(ranges), _at(begin), _at(end), _at(first), _at(lr), *[t.data_ptr() for t in tensors],
         float(betas[0]), float(betas[1]), float(eps), int(step), float(max_norm), norm.data_ptr(),
-        ws.data_ptr(), ws.numel(), _native._stream(tensors[0].device)), "sarr_adam_step_clipped")
+        ws.data_ptr(), ws.numel(), _native._raw_stream(tensors[0].device)), "sarr_adam_step_clipped")

@@ -16,6 +16,7 @@ in 32 bits and rounded once; results are bitwise reproducible. No counterpart
 in the reference, which keeps all SH coefficients of every Gaussian.
 """
 import ctypes
+import functools
 from typing import NamedTuple, Optional
 
 import torch
@@ -47,9 +48,10 @@ def _matrix(t, name):
     if t.dim() != 2:
         raise RuntimeError(f"{name} must be a matrix, got shape {tuple(t.shape)}")
     rows, cols = t.shape
-    if (cols > 1 and t.stride(1) != 1) or (rows > 1 and t.stride(0) < cols):
-        t = t.contiguous()
-    return t, max(t.stride(0), cols) if rows > 1 else cols
+    stride, step = t.stride()
+    if (cols > 1 and step != 1) or (rows > 1 and stride < cols):
+        t, stride = t.contiguous(), cols
+    return t, stride if rows > 1 else cols
 
 
 def _index(index, name="index"):
@@ -59,13 +61,12 @@ def _index(index, name="index"):
         raise RuntimeError(f"{name} must be a CUDA tensor (there is no CPU path)")
     if index.dtype not in _INDEX_BITS:
         raise RuntimeError(f"{name} must be int32 or int64, got {index.dtype}")
-    return index.reshape(-1).contiguous()
+    return index if index.is_contiguous() else index.contiguous()
 
 
-def _same_device(dev, **tensors):
-    for name, t in tensors.items():
-        if t.device != dev:
-            raise RuntimeError(f"{name} is on {t.device}, expected {dev}")
+def _same_device(dev, name, t):
+    if t.device != dev:
+        raise RuntimeError(f"{name} is on {t.device}, expected {dev}")
 
 
 def _out_type(dtype, allowed, what):
@@ -74,52 +75,64 @@ def _out_type(dtype, allowed, what):
     return dtype
 
 
-def _size(fn, *args):
+def _check_out(out, rows, cols, dev, name="out"):
+    t, stride = _matrix(out, name)
+    if t is not out or t.shape != (rows, cols):
+        raise RuntimeError(f"{name} must be a matrix of {rows} x {cols} with contiguous rows")
+    _same_device(dev, name, t)
+    return stride
+
+
+@functools.lru_cache(maxsize=1024)
+def _size(name, *args):
+    """Workspace bytes for these sizes."""
     out = ctypes.c_size_t()
-    _native._check(fn(*args, ctypes.byref(out)), fn.__name__)
+    _native._check(getattr(_native.lib(), name)(*args, ctypes.byref(out)), name)
     return out.value
 
 
 def _lookup(table, index, scale, dtype, out=None):
     table, stride = _matrix(table, "table")
-    shape = index.shape
     index = _index(index)
     dev = table.device
-    _same_device(dev, index=index)
+    _same_device(dev, "index", index)
     dtype = _out_type(dtype or table.dtype, (table.dtype, torch.float32), "dtype")
     codes, cols = table.shape
     n = index.numel()
-    if out is None:
-        rows = torch.empty((n, cols), dtype=dtype, device=dev)
-        rows_stride = cols
-    else:
-        rows, rows_stride = _matrix(out, "out")
-        if rows is not out or rows.dtype != dtype or rows.shape != (n, cols):
-            raise RuntimeError(f"out must be a {dtype} matrix of {n} x {cols} with contiguous rows")
-        _same_device(dev, out=rows)
-    with torch.cuda.device(dev):
+    rows_stride = cols
+    if out is not None:
+        rows_stride = _check_out(out, n, cols, dev)
+        if out.dtype != dtype:
+            raise RuntimeError(f"out must be {dtype}, got {out.dtype}")
+    with _native._on(dev):
+        rows = torch.empty((*index.shape, cols), dtype=dtype, device=dev) if out is None else out
         _native._check(_native.lib().sarr_codebook_lookup(
             n, codes, cols, index.data_ptr(), _INDEX_BITS[index.dtype], table.data_ptr(),
             _TYPES[table.dtype], stride, float(scale), rows.data_ptr(), _TYPES[dtype], rows_stride,
-            _native._stream(dev)), "sarr_codebook_lookup")
-    return rows if out is not None else rows.view(*shape, cols)
+            _native._raw_stream(dev)), "sarr_codebook_lookup")
+    return rows
 
 
 def sort_by_code(index: torch.Tensor, codes: int) -> SortedCodes:
     """The stable order of the Gaussians by code (`index` flattened)."""
     index = _index(index)
     dev, n, codes = index.device, index.numel(), int(codes)
-    L = _native.lib()
-    with torch.cuda.device(dev):
-        ws = torch.empty(_size(L.sarr_codebook_sort_workspace_size, n, codes), dtype=torch.uint8, device=dev)
+    size = _size("sarr_codebook_sort_workspace_size", n, codes)
+    with _native._on(dev):
+        ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
         order = torch.empty(n, dtype=torch.int32, device=dev)
         sorted_codes = torch.empty(n, dtype=torch.int32, device=dev)
         offsets = torch.empty(codes + 1, dtype=torch.int32, device=dev)
-        _native._check(L.sarr_codebook_sort(
+        _native._check(_native.lib().sarr_codebook_sort(
             n, codes, index.data_ptr(), _INDEX_BITS[index.dtype], order.data_ptr(),
-            sorted_codes.data_ptr(), offsets.data_ptr(), ws.data_ptr(), ws.numel(),
-            _native._stream(dev)), "sarr_codebook_sort")
+            sorted_codes.data_ptr(), offsets.data_ptr(), ws.data_ptr() if size else None, size,
+            _native._raw_stream(dev)), "sarr_codebook_sort")
     return SortedCodes(order, sorted_codes, offsets)
+
+
+def _gradient_type(rows, dtype):
+    allowed = tuple(_TYPES) if rows.dtype == torch.float32 else (rows.dtype, torch.float32)
+    return _out_type(dtype or rows.dtype, allowed, "dtype")
 
 
 def gradient_sorted(grad_rows: torch.Tensor, sorted_codes: SortedCodes, scale: float = 1.0,
@@ -135,44 +148,52 @@ def gradient_sorted(grad_rows: torch.Tensor, sorted_codes: SortedCodes, scale: f
     for name, t in (("order", order), ("codes", places), ("offsets", offsets)):
         if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous():
             raise RuntimeError(f"sorted_codes.{name} must be a contiguous int32 vector")
-        _same_device(dev, **{f"sorted_codes.{name}": t})
+        _same_device(dev, name, t)
     if order.numel() != n or places.numel() != n or offsets.numel() < 1:
         raise RuntimeError(f"sorted_codes is of {order.numel()} Gaussians, grad_rows of {n}")
     codes = offsets.numel() - 1
-    if out is None:
-        dtype = dtype or rows.dtype
-    elif dtype is not None and dtype != out.dtype:
-        raise RuntimeError(f"out is {out.dtype}, dtype {dtype}")
-    else:
+    stride = cols
+    if out is not None:
+        stride = _check_out(out, codes, cols, dev)
+        if dtype is not None and dtype != out.dtype:
+            raise RuntimeError(f"out is {out.dtype}, dtype {dtype}")
         dtype = out.dtype
-    allowed = tuple(_TYPES) if rows.dtype == torch.float32 else (rows.dtype, torch.float32)
-    dtype = _out_type(dtype, allowed, "dtype")
-    if out is None:
-        table = torch.empty((codes, cols), dtype=dtype, device=dev)
-        stride = cols
-    else:
-        table, stride = _matrix(out, "out")
-        if table is not out or table.shape != (codes, cols):
-            raise RuntimeError(f"out must be a matrix of {codes} x {cols} with contiguous rows")
-        _same_device(dev, out=table)
-    L = _native.lib()
-    with torch.cuda.device(dev):
-        ws = torch.empty(_size(L.sarr_codebook_grad_workspace_size, n, cols), dtype=torch.uint8, device=dev)
-        _native._check(L.sarr_codebook_grad(
+    dtype = _gradient_type(rows, dtype)
+    size = _size("sarr_codebook_grad_workspace_size", n, cols)
+    with _native._on(dev):
+        table = torch.empty((codes, cols), dtype=dtype, device=dev) if out is None else out
+        ws = torch.empty(size, dtype=torch.uint8, device=dev)
+        _native._check(_native.lib().sarr_codebook_grad(
             n, codes, cols, rows.data_ptr(), _TYPES[rows.dtype], rows_stride, order.data_ptr(),
             places.data_ptr(), offsets.data_ptr(), float(scale), table.data_ptr(), _TYPES[dtype], stride,
-            ws.data_ptr(), ws.numel(), _native._stream(dev)), "sarr_codebook_grad")
+            ws.data_ptr(), size, _native._raw_stream(dev)), "sarr_codebook_grad")
     return table
 
 
 def gradient(grad_rows: torch.Tensor, index: torch.Tensor, codes: int, scale: float = 1.0,
              dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """The table's gradient [codes, cols] of lookup(table, index, scale) from the
-    rows' gradients [*index.shape, cols]."""
-    rows = grad_rows.reshape(-1, grad_rows.shape[-1]) if grad_rows.dim() != 2 else grad_rows
-    if rows.shape[0] != index.numel():
-        raise RuntimeError(f"grad_rows has {rows.shape[0]} rows, index {index.numel()} elements")
-    return gradient_sorted(rows, sort_by_code(index, codes), scale, dtype)
+    rows' gradients [*index.shape, cols] (sort_by_code and gradient_sorted in one
+    call)."""
+    if isinstance(grad_rows, torch.Tensor) and grad_rows.dim() > 2:
+        grad_rows = grad_rows.reshape(-1, grad_rows.shape[-1])
+    rows, rows_stride = _matrix(grad_rows, "grad_rows")
+    index = _index(index)
+    dev, codes = rows.device, int(codes)
+    _same_device(dev, "index", index)
+    n, cols = rows.shape
+    if n != index.numel():
+        raise RuntimeError(f"grad_rows has {n} rows, index {index.numel()} elements")
+    dtype = _gradient_type(rows, dtype)
+    size = _size("sarr_codebook_gradient_workspace_size", n, codes, cols)
+    with _native._on(dev):
+        table = torch.empty((codes, cols), dtype=dtype, device=dev)
+        ws = torch.empty(size, dtype=torch.uint8, device=dev)
+        _native._check(_native.lib().sarr_codebook_gradient(
+            n, codes, cols, rows.data_ptr(), _TYPES[rows.dtype], rows_stride, index.data_ptr(),
+            _INDEX_BITS[index.dtype], float(scale), table.data_ptr(), _TYPES[dtype], cols, ws.data_ptr(), size,
+            _native._raw_stream(dev)), "sarr_codebook_gradient")
+    return table
 
 
 class _Lookup(torch.autograd.Function):

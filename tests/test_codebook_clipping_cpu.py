@@ -43,8 +43,8 @@ def _sort(**kw):
 @pytest.mark.parametrize("kw,status", [
     (dict(n=-1), ARG), (dict(n=BIG), ARG), (dict(codes=-1), ARG), (dict(codes=BIG), ARG), (dict(bits=8), ARG),
     (dict(index=None), ARG), (dict(order=None), ARG), (dict(sorted=None), ARG), (dict(offsets=None), ARG),
-    (dict(order=ctypes.c_void_p(258)), ARG), (dict(ws=None), WORKSPACE), (dict(ws_bytes=16), WORKSPACE),
-    (dict(ws=ctypes.c_void_p(264)), WORKSPACE)])
+    (dict(order=ctypes.c_void_p(258)), ARG), (dict(n=20000, ws=None), WORKSPACE), (dict(n=20000, ws_bytes=16), WORKSPACE),
+    (dict(n=20000, ws=ctypes.c_void_p(264)), WORKSPACE)])
 def test_sort_refusals(kw, status):
     assert _sort(**kw) == status
 
@@ -119,9 +119,8 @@ def test_workspace_sizes_grow():
         assert fn(*a, ctypes.byref(out)) == 0
         return out.value
 
-    assert size(L.sarr_codebook_sort_workspace_size, 0, 0) > 0
     # two digits need one buffer of keys and places beside the outputs
-    assert size(L.sarr_codebook_sort_workspace_size, 1_000_000, 4096) >= 8_000_000
+    assert size(L.sarr_codebook_sort_workspace_size, 1_000_000, 65536) >= 8_000_000
     assert size(L.sarr_codebook_grad_workspace_size, 1_000_000, 16) > size(L.sarr_codebook_grad_workspace_size, 1000, 16)
     assert size(L.sarr_grad_norm_workspace_size, 2000) > size(L.sarr_grad_norm_workspace_size, 1)
     assert L.sarr_codebook_sort_workspace_size(-1, 4, ctypes.byref(out)) == ARG
