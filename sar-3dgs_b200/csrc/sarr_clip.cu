@@ -41,8 +41,8 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kVecs = 4;                        // 16-byte loads of a thread for a piece, in flight together
 constexpr int kPieceBytes = kThreads * kVecs * 16;  // of the gradient
-constexpr int kNormCtas = 148 * 4;              // the most CTAs (and partials) of one norm_kernel launch
-constexpr int kClipCtas = 148 * 4, kAdamCtas = 148 * 4;
+constexpr int kNormCtas = 148 * 8;              // the most CTAs (and partials) of one norm_kernel launch
+constexpr int kClipCtas = 148 * 8, kAdamCtas = 148 * 6;
 constexpr int kSmallList = 16, kMediumList = 96, kLargeList = 512;  // tensors of one launch (kernel parameters)
 constexpr int kAdamRanges = 64;
 
@@ -154,46 +154,35 @@ __device__ __forceinline__ int64_t first_piece(const TensorList<kMax>& L, int t)
   return t > 0 ? L.e[t - 1].piece_end : 0;
 }
 
-// The elements of the 16 bytes at element i (numbered as in Entry) that belong to
-// the tensor, one by one.
-template <bool kInf>
-__device__ __forceinline__ double ragged_norm(const Entry& E, int64_t i, int per, double acc) {
-  for (int k = 0; k < per; ++k)
-    if (i + k >= E.lead && i + k < E.lead + E.count)
-      acc = norm_add<kInf>(acc, load_as_float(E.in, E.type, i + k - E.lead));
-  return acc;
-}
-
+// Pieces inside a tensor are read 16 bytes at a time, its first and last one (which
+// begin or end between 16-byte boundaries) element by element.
 template <int kType, bool kInf>
 __device__ __forceinline__ double piece_norm(const Entry& E, int64_t piece, double acc) {
-  constexpr int kPer = kType == SARR_F32 ? 4 : 8;  // elements of 16 bytes
-  const int64_t at = piece * (kThreads * kVecs * kPer), end = E.lead + E.count;
-  const uint4* p = reinterpret_cast<const uint4*>(static_cast<const char*>(E.in) - E.lead * (16 / kPer)) + at / kPer;
-  uint4 q[kVecs];
-  if (at >= E.lead && at + kThreads * kVecs * kPer <= end) {
+  constexpr int kPer = kType == SARR_F32 ? 4 : 8, kElems = kThreads * kVecs * kPer;  // of 16 bytes, of a piece
+  const int64_t at = piece * kElems - E.lead;
+  if (at >= 0 && at + kElems <= E.count) {
+    const uint4* p = reinterpret_cast<const uint4*>(static_cast<const char*>(E.in) + at * (16 / kPer));
+    uint4 q[kVecs];
 #pragma unroll
     for (int k = 0; k < kVecs; ++k) q[k] = p[k * kThreads + threadIdx.x];
-  } else {
 #pragma unroll
     for (int k = 0; k < kVecs; ++k) {
-      const int64_t i = at + (int64_t)(k * kThreads + threadIdx.x) * kPer;
-      q[k] = make_uint4(0, 0, 0, 0);
-      if (i >= E.lead && i + kPer <= end) q[k] = p[k * kThreads + threadIdx.x];
-      else acc = ragged_norm<kInf>(E, i, kPer, acc);
+      float x[8];
+      unpack(q[k], kType, x);
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) acc = norm_add<kInf>(acc, x[j]);
     }
-  }
-#pragma unroll
-  for (int k = 0; k < kVecs; ++k) {
-    float x[8];
-    unpack(q[k], kType, x);
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) acc = norm_add<kInf>(acc, x[j]);
+  } else {
+    const int64_t end = min(at + kElems, E.count);
+#pragma unroll 4
+    for (int64_t i = max(at, (int64_t)0) + threadIdx.x; i < end; i += kThreads)
+      acc = norm_add<kInf>(acc, load_as_float(E.in, kType, i));
   }
   return acc;
 }
 
 template <int kMax, bool kInf>
-__global__ void __launch_bounds__(kThreads) norm_kernel(const __grid_constant__ TensorList<kMax> L,
+__global__ void __launch_bounds__(kThreads, 8) norm_kernel(const __grid_constant__ TensorList<kMax> L,
                                                         double* __restrict__ partial) {
   sarr::dependents_may_start();
   sarr::wait_for_previous();
@@ -273,37 +262,24 @@ template <int kIn, int kOut>
 __device__ __forceinline__ void piece_clip(const Entry& E, int64_t piece, float c) {
   constexpr int kPer = kIn == SARR_F32 ? 4 : 8, kOutSize = kOut == SARR_F32 ? 4 : 2;
   constexpr int kElems = kThreads * kVecs * kPer;
-  const int64_t at = piece * kElems, end = E.lead + E.count;
-  if (!E.vec) {  // out is aligned otherwise than in: element by element
-    for (int v = threadIdx.x; v < kElems; v += kThreads) {
-      const int64_t i = at + v - E.lead;
-      if (i >= 0 && i < E.count) store_float(E.out, kOut, i, load_as_float(E.in, kIn, i) * c);
-    }
-    return;
-  }
-  const uint4* p = reinterpret_cast<const uint4*>(static_cast<const char*>(E.in) - E.lead * (16 / kPer)) + at / kPer;
-  char* o = static_cast<char*>(E.out) + (at - E.lead) * kOutSize;
-  const bool whole = at >= E.lead && at + kElems <= end;
-  uint4 q[kVecs];
+  const int64_t at = piece * kElems - E.lead;
+  if (E.vec && at >= 0 && at + kElems <= E.count) {
+    const uint4* p = reinterpret_cast<const uint4*>(static_cast<const char*>(E.in) + at * (16 / kPer));
+    char* o = static_cast<char*>(E.out) + at * kOutSize;
+    uint4 q[kVecs];
 #pragma unroll
-  for (int k = 0; k < kVecs; ++k) {
-    const int64_t i = at + (int64_t)(k * kThreads + threadIdx.x) * kPer;
-    if (whole || (i >= E.lead && i + kPer <= end)) q[k] = p[k * kThreads + threadIdx.x];
-  }
+    for (int k = 0; k < kVecs; ++k) q[k] = p[k * kThreads + threadIdx.x];
 #pragma unroll
-  for (int k = 0; k < kVecs; ++k) {
-    const int v = k * kThreads + threadIdx.x;
-    const int64_t i = at + (int64_t)v * kPer;
-    if (whole || (i >= E.lead && i + kPer <= end)) {
+    for (int k = 0; k < kVecs; ++k) {
       float x[8];
       unpack(q[k], kIn, x);
-      store_scaled<kOut>(o + (int64_t)v * kPer * kOutSize, x, kPer, c);
-    } else {
-      for (int j = 0; j < kPer; ++j) {
-        const int64_t e = i + j - E.lead;
-        if (e >= 0 && e < E.count) store_float(E.out, kOut, e, load_as_float(E.in, kIn, e) * c);
-      }
+      store_scaled<kOut>(o + (k * kThreads + (int)threadIdx.x) * kPer * kOutSize, x, kPer, c);
     }
+  } else {  // a tensor's first or last piece, or out is aligned otherwise than in
+    const int64_t end = min(at + kElems, E.count);
+#pragma unroll 4
+    for (int64_t i = max(at, (int64_t)0) + threadIdx.x; i < end; i += kThreads)
+      store_float(E.out, kOut, i, load_as_float(E.in, kIn, i) * c);
   }
 }
 
@@ -313,7 +289,7 @@ __device__ __forceinline__ void clip_run(const Entry& E, int64_t from, int64_t t
 }
 
 template <int kMax, bool kInf>
-__global__ void __launch_bounds__(kThreads) clip_kernel(const __grid_constant__ TensorList<kMax> L,
+__global__ void __launch_bounds__(kThreads, 8) clip_kernel(const __grid_constant__ TensorList<kMax> L,
                                                         const double* __restrict__ partial, int n_partial,
                                                         double max_norm, float* __restrict__ norm_out) {
   sarr::wait_for_previous();
@@ -339,7 +315,7 @@ __global__ void __launch_bounds__(kThreads) clip_kernel(const __grid_constant__ 
 // ---------------------------------------------------------------------------
 // Adam
 // ---------------------------------------------------------------------------
-constexpr int kAdamVecs = 2, kAdamPiece = kThreads * kAdamVecs * 4;  // elements
+constexpr int kAdamVecs = 1, kAdamPiece = kThreads * kAdamVecs * 4;  // elements
 
 struct AdamRange {
   int64_t begin, count;  // elements of param / exp_avg / exp_avg_sq
@@ -367,7 +343,7 @@ __device__ __forceinline__ float adam_one(const AdamList& A, float step_size, fl
   return __fadd_rn(p, __fmul_rn(-step_size, __fdiv_rn(m, denom)));
 }
 
-__global__ void __launch_bounds__(kThreads) adam_kernel(const __grid_constant__ AdamList A,
+__global__ void __launch_bounds__(kThreads, 6) adam_kernel(const __grid_constant__ AdamList A,
                                                         const double* __restrict__ partial, int n_partial,
                                                         double max_norm, float* __restrict__ param,
                                                         const float* __restrict__ grad,

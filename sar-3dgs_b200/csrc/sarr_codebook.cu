@@ -27,9 +27,6 @@ void count_launches(int k);  // the library's launch counter (sarr_abi.cu)
 
 namespace {
 
-__device__ __forceinline__ float to_float(float x) { return x; }
-__device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
-__device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
 template <typename T>
 __device__ __forceinline__ T from_float(float x);
 template <>
@@ -45,29 +42,50 @@ __device__ __forceinline__ W load_word(const W* p) {
   return kAgain ? __ldg(p) : __ldcg(p);
 }
 
-// kV consecutive elements as floats; p is aligned to min(16, kV * sizeof(T)) bytes.
+// kV consecutive elements as they lie in memory (floats of them only where they
+// are used: half the registers of a 16-bit row in flight).
+template <typename T, int kV>
+struct Raw {
+  static constexpr int kBytes = kV * (int)sizeof(T), kWords = (kBytes + 3) / 4;
+  uint32_t w[kWords];
+};
+
+// p is aligned to min(16, kV * sizeof(T)) bytes.
 template <bool kAgain, typename T, int kV>
-__device__ __forceinline__ void load_vec(const T* p, float (&x)[kV]) {
-  constexpr int kBytes = kV * (int)sizeof(T);
-  T t[kV];
+__device__ __forceinline__ Raw<T, kV> load_raw(const T* p) {
+  constexpr int kBytes = Raw<T, kV>::kBytes;
+  Raw<T, kV> x;
   if constexpr (kBytes >= 16) {
 #pragma unroll
     for (int k = 0; k < kBytes / 16; ++k) {
       const uint4 q = load_word<kAgain>(reinterpret_cast<const uint4*>(p) + k);
-      memcpy(reinterpret_cast<char*>(t) + 16 * k, &q, 16);
+      x.w[4 * k] = q.x, x.w[4 * k + 1] = q.y, x.w[4 * k + 2] = q.z, x.w[4 * k + 3] = q.w;
     }
   } else if constexpr (kBytes == 8) {
     const uint2 q = load_word<kAgain>(reinterpret_cast<const uint2*>(p));
-    memcpy(t, &q, 8);
+    x.w[0] = q.x, x.w[1] = q.y;
   } else if constexpr (kBytes == 4) {
-    const unsigned q = load_word<kAgain>(reinterpret_cast<const unsigned*>(p));
-    memcpy(t, &q, 4);
+    x.w[0] = load_word<kAgain>(reinterpret_cast<const unsigned*>(p));
   } else {
-    const unsigned short q = load_word<kAgain>(reinterpret_cast<const unsigned short*>(p));
-    memcpy(t, &q, 2);
+    x.w[0] = load_word<kAgain>(reinterpret_cast<const unsigned short*>(p));
   }
+  return x;
+}
+
+template <int kV>
+__device__ __forceinline__ void to_floats(const Raw<float, kV>& r, float (&x)[kV]) {
 #pragma unroll
-  for (int k = 0; k < kV; ++k) x[k] = to_float(t[k]);
+  for (int k = 0; k < kV; ++k) x[k] = __uint_as_float(r.w[k]);
+}
+template <int kV>
+__device__ __forceinline__ void to_floats(const Raw<__nv_bfloat16, kV>& r, float (&x)[kV]) {
+#pragma unroll
+  for (int k = 0; k < kV; ++k) x[k] = __uint_as_float(k & 1 ? r.w[k / 2] & 0xffff0000u : r.w[k / 2] << 16);
+}
+template <int kV>
+__device__ __forceinline__ void to_floats(const Raw<__half, kV>& r, float (&x)[kV]) {
+#pragma unroll
+  for (int k = 0; k < kV; ++k) x[k] = __half2float(__ushort_as_half((unsigned short)(r.w[k / 2] >> (16 * (k & 1)))));
 }
 
 template <typename T, int kV>
@@ -97,6 +115,11 @@ __device__ __forceinline__ void store_vec(T* p, const float (&x)[kV]) {
 }
 
 // index[i], or `codes` where it is outside [0, codes).
+template <typename TI>
+__device__ __forceinline__ uint32_t code_of(const TI* index, int i, uint32_t codes) {
+  const TI v = __ldg(index + i);
+  return v >= 0 && v < (TI)codes ? (uint32_t)v : codes;
+}
 __device__ __forceinline__ uint32_t code_of(const void* index, bool wide, int64_t i, uint32_t codes) {
   const int64_t v = wide ? __ldg(static_cast<const long long*>(index) + i)
                          : (int64_t)__ldg(static_cast<const int*>(index) + i);
@@ -107,51 +130,49 @@ __device__ __forceinline__ uint32_t code_of(const void* index, bool wide, int64_
 // lookup
 // ---------------------------------------------------------------------------
 constexpr int kLookupThreads = 256;
-constexpr int kLookupRows = 4;  // rows per thread, their loads in flight together
+constexpr int kLookupRows = 8;  // rows per thread, their loads in flight together
 
 struct LookupArgs {
   int64_t n;
   uint32_t codes;
   int vecs;    // vectors per row
   int lanes;   // threads per row (a power of two)
-  bool wide;   // 64-bit indexes
   float scale;
   const void* index;
   const void* table;
   void* rows;
-  int64_t table_stride, rows_stride;
+  int64_t table_stride, rows_stride;  // bytes
 };
 
-template <typename TT, typename TR, int kV>
+template <typename TI, typename TT, typename TR, int kV>
 __global__ void __launch_bounds__(kLookupThreads) lookup_kernel(const LookupArgs a) {
   const int lane = threadIdx.x & (a.lanes - 1), at_once = kLookupThreads / a.lanes;
   const int64_t i0 = (int64_t)blockIdx.x * at_once * kLookupRows + threadIdx.x / a.lanes;
+  const int64_t left = a.n - i0;  // row k is there where k * at_once < left
+  const TI* index = static_cast<const TI*>(a.index) + i0;
   uint32_t code[kLookupRows];
 #pragma unroll
-  for (int k = 0; k < kLookupRows; ++k) {
-    const int64_t i = i0 + (int64_t)k * at_once;
-    code[k] = i < a.n ? code_of(a.index, a.wide, i, a.codes) : a.codes;
-  }
+  for (int k = 0; k < kLookupRows; ++k) code[k] = k * at_once < left ? code_of(index, k * at_once, a.codes) : a.codes;
+  const int64_t step = a.rows_stride * at_once;
   for (int v = lane; v < a.vecs; v += a.lanes) {
-    float x[kLookupRows][kV];
+    const char* from = static_cast<const char*>(a.table) + v * (kV * (int)sizeof(TT));
+    char* to = static_cast<char*>(a.rows) + i0 * a.rows_stride + v * (kV * (int)sizeof(TR));
+    Raw<TT, kV> raw[kLookupRows];
 #pragma unroll
-    for (int k = 0; k < kLookupRows; ++k) {
+    for (int k = 0; k < kLookupRows; ++k)
+      if (code[k] < a.codes) raw[k] = load_raw<true, TT, kV>(reinterpret_cast<const TT*>(from + code[k] * a.table_stride));
+#pragma unroll
+    for (int k = 0; k < kLookupRows; ++k, to += step) {
+      float x[kV];
       if (code[k] < a.codes) {
-        load_vec<true, TT, kV>(static_cast<const TT*>(a.table) + code[k] * a.table_stride + (int64_t)v * kV, x[k]);
-      } else {
+        to_floats(raw[k], x);
 #pragma unroll
-        for (int j = 0; j < kV; ++j) x[k][j] = 0.0f;
+        for (int j = 0; j < kV; ++j) x[j] *= a.scale;
+      } else {  // a row without a code is zeros whatever the scale
+#pragma unroll
+        for (int j = 0; j < kV; ++j) x[j] = 0.0f;
       }
-    }
-#pragma unroll
-    for (int k = 0; k < kLookupRows; ++k) {
-      const int64_t i = i0 + (int64_t)k * at_once;
-      if (i >= a.n) continue;
-      if (code[k] < a.codes) {  // a row without a code is zeros whatever the scale
-#pragma unroll
-        for (int j = 0; j < kV; ++j) x[k][j] *= a.scale;
-      }
-      store_vec<TR, kV>(static_cast<TR*>(a.rows) + i * a.rows_stride + (int64_t)v * kV, x[k]);
+      if (k * at_once < left) store_vec<TR, kV>(reinterpret_cast<TR*>(to), x);
     }
   }
 }
@@ -160,13 +181,14 @@ __global__ void __launch_bounds__(kLookupThreads) lookup_kernel(const LookupArgs
 // sort
 // ---------------------------------------------------------------------------
 // A stable sort of the keys (the codes, `codes` for none). The unit is a tile of
-// up to 8192 keys that one CTA sorts in registers and shared memory: each warp
+// 1024 to 8192 keys that one CTA sorts in registers and shared memory: each warp
 // holds a contiguous part of the tile, 32 keys a round; a key's rank among the
 // warp's keys of its digit is a running count plus the lower lanes that vote for
-// the same digit (one vote per bit, so a digit of 7 bits costs 7 votes whatever
-// the keys are), and one scan over (digit, warp) gives every rank its place.
+// the same digit (one vote per bit, so a digit costs the same whatever the keys
+// are), and a scan over the warps' counts and the digits gives every rank its
+// place. Counts are 16 bits wide, two digits to a word.
 //
-// Up to 8192 keys: one CTA, every digit, and the offsets (sort_tile_kernel).
+// One tile: one CTA sorts by every digit and finds the offsets (sort_tile_kernel).
 //
 // More: passes over digits of up to 13 bits (so one pass up to 8191 codes), of
 // three kernels each, which the scheduler may overlap:
@@ -177,12 +199,11 @@ __global__ void __launch_bounds__(kLookupThreads) lookup_kernel(const LookupArgs
 //              first pass sorts its tile before it waits for the other two.
 // With one pass the scan over the totals is the offsets.
 constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32;
-constexpr int kTileRounds = 8, kTile = kSortThreads * kTileRounds;
-constexpr int kLocalBits = 7;                          // of a pass inside a tile
+constexpr int kMaxRounds = 8;                          // keys per thread
+constexpr int kLocalBits = 9, kLocalBins = 1 << kLocalBits;  // of a pass inside a tile, at most
 constexpr int kMaxDigitBits = 13, kMaxBins = 1 << kMaxDigitBits;
-constexpr int kCountPitch = kSortWarps + 1;            // [digit][warp], padded against bank conflicts
-constexpr int kCountWords = kCountPitch << kLocalBits;
 constexpr int kPrefixThreads = 256, kPrefixBins = 32;  // bins of a CTA; its threads split the tiles 8 ways
+constexpr int kManyTiles = 148;                        // tiles grow until there are no more of them than SMs
 
 struct SortArgs {
   int n;
@@ -199,134 +220,145 @@ struct SortArgs {
   int32_t* offsets;          // written by the scatter of a sort of one pass, else null
 };
 
+template <int kRounds>
 struct TileShared {
-  uint32_t key[kTile];
-  int32_t place[kTile];
-  int32_t count[kCountWords];
+  uint32_t key[kSortThreads * kRounds];
+  int32_t place[kSortThreads * kRounds];
+  uint16_t count[kSortWarps][kLocalBins];
+  int32_t digit[kLocalBins];
   int32_t warp_sum[kSortWarps];
 };
 
-// Exclusive scan over the CTA's threads.
-__device__ __forceinline__ int block_scan(int x, int32_t* warp_sum) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int incl = x;
+__device__ __forceinline__ int warp_inclusive(int x, int lane) {
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int y = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += y;
+    const int y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
   }
-  if (lane == 31) warp_sum[warp] = incl;
-  __syncthreads();
-  int before = lane < warp ? warp_sum[lane] : 0;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
-  __syncthreads();
-  return before + incl - x;
+  return x;
+}
+
+// Sum of warp_sum over the warps before this one.
+__device__ __forceinline__ int warps_before(const int32_t* warp_sum, int lane, int warp) {
+  return __reduce_add_sync(0xffffffffu, lane < warp ? warp_sum[lane] : 0);
 }
 
 // One stable pass over the tile's keys, which the threads hold: element
-// (warp * rounds + r) * 32 + lane in key[r]. On return S holds the tile in order
-// and so do the threads.
-__device__ __forceinline__ void tile_pass(TileShared& S, uint32_t (&key)[kTileRounds], int32_t (&place)[kTileRounds],
-                                          int rounds, int len, int shift, int bits) {
+// (warp * kRounds + r) * 32 + lane in key[r]; elements from len on are none. On
+// return S holds the tile in order and so do the threads.
+template <int kRounds>
+__device__ __forceinline__ void tile_pass(TileShared<kRounds>& S, uint32_t (&key)[kRounds], int32_t (&place)[kRounds],
+                                          int len, int shift, int bits) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, bins = 1 << bits;
-  for (int i = tid; i < bins * kCountPitch; i += kSortThreads) S.count[i] = 0;
+  const int first = warp * kRounds * 32 + lane;
+  uint16_t* count = S.count[warp];
+  for (int i = lane; i < (bins + 1) / 2; i += 32) reinterpret_cast<uint32_t*>(count)[i] = 0;
+  uint32_t peers[kRounds];
+#pragma unroll
+  for (int r = 0; r < kRounds; ++r) peers[r] = __ballot_sync(0xffffffffu, first + 32 * r < len);
+  for (int b = 0; b < bits; ++b) {
+#pragma unroll
+    for (int r = 0; r < kRounds; ++r) {
+      const bool one = (key[r] >> (shift + b)) & 1;
+      const uint32_t ones = __ballot_sync(0xffffffffu, one);
+      peers[r] &= one ? ones : ~ones;
+    }
+  }
+  __syncwarp();
+  int rank[kRounds];
+#pragma unroll
+  for (int r = 0; r < kRounds; ++r) {
+    const uint32_t digit = (key[r] >> shift) & (bins - 1), below = peers[r] & ((1u << lane) - 1);
+    const bool have = first + 32 * r < len;
+    const int before = have ? count[digit] : 0;
+    __syncwarp();
+    if (have && below == 0) count[digit] = (uint16_t)(before + __popc(peers[r]));
+    __syncwarp();
+    rank[r] = before + __popc(below);
+  }
   __syncthreads();
-  int rank[kTileRounds];
-#pragma unroll
-  for (int r = 0; r < kTileRounds; ++r) {
-    if (r < rounds) {
-      const bool have = (warp * rounds + r) * 32 + lane < len;
-      const uint32_t digit = (key[r] >> shift) & (bins - 1);
-      uint32_t peers = __ballot_sync(0xffffffffu, have);
-#pragma unroll
-      for (int b = 0; b < kLocalBits; ++b) {  // the bits above `bits` are 0 in every lane
-        const bool one = (digit >> b) & 1;
-        const uint32_t ones = __ballot_sync(0xffffffffu, one);
-        peers &= one ? ones : ~ones;
+  // per digit (two to a thread): the counts of the earlier warps, and the digits before
+  const int pairs = (bins + 1) / 2;
+  int lo = 0, incl = 0;
+  if (tid < ((pairs + 31) & ~31)) {
+    uint32_t sum = 0;
+    if (tid < pairs) {
+#pragma unroll 8
+      for (int w = 0; w < kSortWarps; ++w) {
+        uint32_t* c = reinterpret_cast<uint32_t*>(S.count[w]) + tid;
+        const uint32_t x = *c;
+        *c = sum;
+        sum += x;
       }
-      const uint32_t below = peers & ((1u << lane) - 1);
-      int32_t* at = S.count + digit * kCountPitch + warp;
-      const int before = have ? *at : 0;
-      __syncwarp();
-      if (have && below == 0) *at = before + __popc(peers);
-      __syncwarp();
-      rank[r] = before + __popc(below);
     }
+    lo = sum & 0xffffu;
+    const int both = lo + (int)(sum >> 16);
+    incl = warp_inclusive(both, lane);
+    if (lane == 31) S.warp_sum[warp] = incl;
+    incl -= both;
   }
   __syncthreads();
-  {  // scan in the order (digit, warp): bins / 32 entries per thread, at least one
-    const int each = bins >= 32 ? bins / 32 : 1, first = tid * each;
-    int x[(1 << kLocalBits) / 32], sum = 0;
-#pragma unroll
-    for (int k = 0; k < (1 << kLocalBits) / 32; ++k) {
-      const int e = first + k;
-      x[k] = k < each && e < bins * 32 ? S.count[(e >> 5) * kCountPitch + (e & 31)] : 0;
-      sum += x[k];
-    }
-    int at = block_scan(sum, S.warp_sum);
-#pragma unroll
-    for (int k = 0; k < (1 << kLocalBits) / 32; ++k) {
-      const int e = first + k;
-      if (k < each && e < bins * 32) S.count[(e >> 5) * kCountPitch + (e & 31)] = at;
-      at += x[k];
+  if (tid < ((pairs + 31) & ~31)) {
+    const int at = incl + warps_before(S.warp_sum, lane, warp);
+    if (tid < pairs) {
+      S.digit[2 * tid] = at;
+      if (2 * tid + 1 < bins) S.digit[2 * tid + 1] = at + lo;
     }
   }
   __syncthreads();
 #pragma unroll
-  for (int r = 0; r < kTileRounds; ++r) {
-    if (r < rounds && (warp * rounds + r) * 32 + lane < len) {
-      const int to = S.count[((key[r] >> shift) & (bins - 1)) * kCountPitch + warp] + rank[r];
+  for (int r = 0; r < kRounds; ++r) {
+    if (first + 32 * r < len) {
+      const uint32_t digit = (key[r] >> shift) & (bins - 1);
+      const int to = S.digit[digit] + count[digit] + rank[r];
       S.key[to] = key[r];
       S.place[to] = place[r];
     }
   }
   __syncthreads();
 #pragma unroll
-  for (int r = 0; r < kTileRounds; ++r) {
-    const int e = (warp * rounds + r) * 32 + lane;
-    if (r < rounds && e < len) {
-      key[r] = S.key[e];
-      place[r] = S.place[e];
+  for (int r = 0; r < kRounds; ++r) {
+    if (first + 32 * r < len) {
+      key[r] = S.key[first + 32 * r];
+      place[r] = S.place[first + 32 * r];
     }
   }
 }
 
 // The tile's keys into the threads, then sorted by `bits` bits from `shift`.
-__device__ __forceinline__ void sort_tile(const SortArgs& a, TileShared& S, uint32_t (&key)[kTileRounds],
-                                          int32_t (&place)[kTileRounds], int tile0, int len, int rounds, int shift,
-                                          int bits) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+template <int kRounds>
+__device__ __forceinline__ void sort_tile(const SortArgs& a, TileShared<kRounds>& S, uint32_t (&key)[kRounds],
+                                          int32_t (&place)[kRounds], int tile0, int len, int shift, int bits) {
+  const int first = (threadIdx.x >> 5) * kRounds * 32 + (threadIdx.x & 31);
 #pragma unroll
-  for (int r = 0; r < kTileRounds; ++r) {
-    const int e = (warp * rounds + r) * 32 + lane;
+  for (int r = 0; r < kRounds; ++r) {
+    const int e = first + 32 * r, i = tile0 + e;
     key[r] = 0;
     place[r] = 0;
-    if (r < rounds && e < len) {
-      const int i = tile0 + e;
+    if (e < len) {
       key[r] = a.key_in ? __ldcg(a.key_in + i) : code_of(a.index, a.wide, i, a.codes);
       place[r] = a.key_in ? __ldcg(a.place_in + i) : i;
     }
   }
   const int passes = (bits + kLocalBits - 1) / kLocalBits, each = (bits + passes - 1) / passes;
-  for (int p = 0; p < passes; ++p)
-    tile_pass(S, key, place, rounds, len, shift + p * each, min(each, bits - p * each));
+#pragma unroll 1
+  for (int p = 0; p < passes; ++p) tile_pass<kRounds>(S, key, place, len, shift + p * each, min(each, bits - p * each));
 }
 
 extern __shared__ __align__(16) unsigned char s_sort[];
 
+template <int kRounds>
 __global__ void __launch_bounds__(kSortThreads) sort_tile_kernel(const SortArgs a) {
-  TileShared& S = *reinterpret_cast<TileShared*>(s_sort);
-  uint32_t key[kTileRounds];
-  int32_t place[kTileRounds];
+  TileShared<kRounds>& S = *reinterpret_cast<TileShared<kRounds>*>(s_sort);
+  uint32_t key[kRounds];
+  int32_t place[kRounds];
   sarr::dependents_may_start();
-  const int rounds = (a.n + kSortThreads - 1) / kSortThreads;
-  sort_tile(a, S, key, place, 0, a.n, rounds, 0, a.bits);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  sort_tile<kRounds>(a, S, key, place, 0, a.n, 0, a.bits);
+  const int first = (threadIdx.x >> 5) * kRounds * 32 + (threadIdx.x & 31);
 #pragma unroll
-  for (int r = 0; r < kTileRounds; ++r) {
-    const int e = (warp * rounds + r) * 32 + lane;
-    if (r < rounds && e < a.n) {
+  for (int r = 0; r < kRounds; ++r) {
+    const int e = first + 32 * r;
+    if (e < a.n) {
       a.key_out[e] = key[r];
       a.place_out[e] = place[r];
     }
@@ -344,21 +376,23 @@ __global__ void __launch_bounds__(kSortThreads) sort_tile_kernel(const SortArgs 
   }
 }
 
+template <int kRounds>
 __global__ void __launch_bounds__(kSortThreads) sort_histogram_kernel(const SortArgs a) {
+  constexpr int kTile = kSortThreads * kRounds;
   __shared__ int32_t s_bin[kMaxBins];
   sarr::dependents_may_start();
   sarr::wait_for_previous();
   const int bins = 1 << a.bits, tile0 = blockIdx.x * kTile, len = min(kTile, a.n - tile0);
-  for (int d = threadIdx.x; d < bins; d += kSortThreads) s_bin[d] = 0;
-  uint32_t key[kTileRounds];
+  uint32_t key[kRounds];
 #pragma unroll
-  for (int r = 0; r < kTileRounds; ++r) {
+  for (int r = 0; r < kRounds; ++r) {
     const int e = r * kSortThreads + threadIdx.x;
     if (e < len) key[r] = a.key_in ? __ldcg(a.key_in + tile0 + e) : code_of(a.index, a.wide, tile0 + e, a.codes);
   }
+  for (int d = threadIdx.x; d < bins; d += kSortThreads) s_bin[d] = 0;
   __syncthreads();
 #pragma unroll
-  for (int r = 0; r < kTileRounds; ++r)
+  for (int r = 0; r < kRounds; ++r)
     if (r * kSortThreads + threadIdx.x < len) atomicAdd(s_bin + ((key[r] >> a.shift) & (bins - 1)), 1);
   __syncthreads();
   for (int d = threadIdx.x; d < bins; d += kSortThreads) a.counts[(int64_t)blockIdx.x * bins + d] = s_bin[d];
@@ -402,34 +436,36 @@ __global__ void __launch_bounds__(kPrefixThreads) sort_prefix_kernel(const SortA
   }
 }
 
+template <int kRounds>
 __global__ void __launch_bounds__(kSortThreads) sort_scatter_kernel(const SortArgs a) {
-  TileShared& S = *reinterpret_cast<TileShared*>(s_sort);
-  int32_t* s_base = reinterpret_cast<int32_t*>(s_sort + sizeof(TileShared));  // [bins]
-  uint32_t key[kTileRounds];
-  int32_t place[kTileRounds];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  constexpr int kTile = kSortThreads * kRounds, kBinsEach = kMaxBins / kSortThreads;
+  TileShared<kRounds>& S = *reinterpret_cast<TileShared<kRounds>*>(s_sort);
+  int32_t* s_base = reinterpret_cast<int32_t*>(s_sort + sizeof(TileShared<kRounds>));  // [bins]
+  uint32_t key[kRounds];
+  int32_t place[kRounds];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, begin = warp * kRounds * 32 + lane;
   const int bins = 1 << a.bits, tile0 = blockIdx.x * kTile, len = min(kTile, a.n - tile0);
-  const int rounds = (len + kSortThreads - 1) / kSortThreads;
   sarr::dependents_may_start();
   if (a.key_in) sarr::wait_for_previous();  // the first pass's keys are the caller's
-  sort_tile(a, S, key, place, tile0, len, rounds, a.shift, a.bits);
+  sort_tile<kRounds>(a, S, key, place, tile0, len, a.shift, a.bits);
   if (!a.key_in) sarr::wait_for_previous();
   // where each digit begins, and in it this tile's keys
   {
     const int each = max(bins / kSortThreads, 1), first = tid * each;
-    int x[kMaxBins / kSortThreads], sum = 0;
+    int x[kBinsEach], before[kBinsEach], sum = 0;
 #pragma unroll
-    for (int k = 0; k < kMaxBins / kSortThreads; ++k) {
-      x[k] = k < each && first + k < bins ? __ldcg(a.totals + first + k) : 0;
+    for (int k = 0; k < kBinsEach; ++k) {
+      const bool have = k < each && first + k < bins;
+      x[k] = have ? __ldcg(a.totals + first + k) : 0;
+      before[k] = have ? __ldcg(a.counts + (int64_t)blockIdx.x * bins + first + k) : 0;
       sum += x[k];
     }
-    int before[kMaxBins / kSortThreads];
+    const int incl = warp_inclusive(sum, lane);
+    if (lane == 31) S.warp_sum[warp] = incl;
+    __syncthreads();
+    int at = incl - sum + warps_before(S.warp_sum, lane, warp);
 #pragma unroll
-    for (int k = 0; k < kMaxBins / kSortThreads; ++k)
-      before[k] = k < each && first + k < bins ? __ldcg(a.counts + (int64_t)blockIdx.x * bins + first + k) : 0;
-    int at = block_scan(sum, S.warp_sum);
-#pragma unroll
-    for (int k = 0; k < kMaxBins / kSortThreads; ++k) {
+    for (int k = 0; k < kBinsEach; ++k) {
       const int d = first + k;
       if (k < each && d < bins) {
         s_base[d] = at + before[k];
@@ -441,18 +477,18 @@ __global__ void __launch_bounds__(kSortThreads) sort_scatter_kernel(const SortAr
   __syncthreads();
   // less the place in the tile where the digit begins
 #pragma unroll
-  for (int r = 0; r < kTileRounds; ++r) {
-    const int e = (warp * rounds + r) * 32 + lane;
-    if (r < rounds && e < len) {
+  for (int r = 0; r < kRounds; ++r) {
+    const int e = begin + 32 * r;
+    if (e < len) {
       const uint32_t d = (key[r] >> a.shift) & (bins - 1);
       if (e == 0 || ((S.key[e - 1] >> a.shift) & (bins - 1)) != d) s_base[d] -= e;
     }
   }
   __syncthreads();
 #pragma unroll
-  for (int r = 0; r < kTileRounds; ++r) {
-    const int e = (warp * rounds + r) * 32 + lane;
-    if (r < rounds && e < len) {
+  for (int r = 0; r < kRounds; ++r) {
+    const int e = begin + 32 * r;
+    if (e < len) {
       const int to = s_base[(key[r] >> a.shift) & (bins - 1)] + e;
       a.key_out[to] = key[r];
       a.place_out[to] = place[r];
@@ -484,19 +520,23 @@ __global__ void __launch_bounds__(256) sort_offsets_kernel(int n, uint32_t codes
 // side by side: equal work whatever the codes' lengths. A group adds the rows
 // of its part in order and writes the codes that lie inside it; the sums of
 // codes that cross a part's border are joined through shared memory, those of
-// codes that cross a span's border through the workspace, by grad_finish_kernel,
-// which also writes the zeros of codes without Gaussians.
+// codes that cross a span's border through the workspace, by grad_finish_kernel.
+// CTAs behind the spans' write the zeros of the codes without Gaussians, while
+// the others wait for their rows.
 constexpr int kGradThreads = 256;
 constexpr int kGradRows = 8;     // rows of a group loaded together
 constexpr int kMaxPart = 64;     // places of a group, at most
 constexpr int kMaxSpan = 2048;   // places of a CTA, at most
+constexpr int kGradCtas = 148 * 3;  // parts grow while there are as many CTAs
+constexpr int kFillCodes = 8;    // codes of a group in a zero-writing CTA
 constexpr int kLongSpans = 16;   // spans from which a code's partials are added by a whole CTA
 
 struct GradArgs {
+  int n;
   int64_t cols;
   uint32_t codes;
   int vecs, lanes, part;  // vectors per row; threads per row; places per group
-  int span;               // places per CTA: part * (kGradThreads / lanes)
+  int span, spans;        // places per CTA: part * (kGradThreads / lanes); CTAs with places
   float scale;
   const void* rows;
   int64_t rows_stride;
@@ -514,98 +554,139 @@ __device__ __forceinline__ void write_row(const GradArgs& a, uint32_t code, int 
   store_vec<TT, kV>(static_cast<TT*>(a.table) + code * a.table_stride + (int64_t)v * kV, x);
 }
 
+// Partials are at [span][slot][v][j]: kV floats side by side.
 template <int kV>
-__device__ __forceinline__ void write_partial(const GradArgs& a, int span, int slot, int v, const float (&x)[kV]) {
-  float* p = a.partial + ((int64_t)span * 2 + slot) * a.cols + (int64_t)v * kV;
-#pragma unroll
-  for (int j = 0; j < kV; ++j) p[j] = x[j];
+__device__ __forceinline__ float* partial_at(const GradArgs& a, int span, int slot, int v) {
+  return a.partial + ((int64_t)span * 2 + slot) * a.cols + (int64_t)v * kV;
 }
 
 template <typename TG, typename TT, int kV>
-__global__ void __launch_bounds__(kGradThreads) grad_kernel(const GradArgs a) {
-  __shared__ int32_t s_code[kMaxSpan + 2];  // codes of the span, with its neighbours
-  __shared__ int32_t s_row[kMaxSpan];
+__global__ void __launch_bounds__(kGradThreads, 4) grad_kernel(const GradArgs a) {
+  // codes and rows of the parts, each part kPad words behind the one before, so
+  // that groups at the same place of their parts use different banks
+  constexpr int kPad = 4, kWords = kMaxSpan + kMaxSpan / kGradRows * kPad;
+  __shared__ __align__(16) int32_t s_code[kWords], s_row[kWords];
   __shared__ float s_head[kV][kGradThreads], s_tail[kV][kGradThreads];
   __shared__ uint8_t s_state[kGradThreads];  // per group
+  __shared__ int32_t s_edge[2];              // codes before and behind the span
   enum : uint8_t { kHead = 1, kTail = 2, kThrough = 4 };
   sarr::dependents_may_start();
   sarr::wait_for_previous();
 
   const int tid = threadIdx.x, lane = tid & (a.lanes - 1), group = tid / a.lanes;
   const int groups = kGradThreads / a.lanes;
-  const int n = a.offsets[a.codes];  // places with a code
-  const int64_t p0 = (int64_t)blockIdx.x * a.span;
-  if (p0 >= n) return;
-  const int len = (int)(n - p0 < a.span ? n - p0 : a.span);
-  for (int i = tid; i < len + 2; i += kGradThreads) {
-    const int64_t p = p0 + i - 1;
-    s_code[i] = p >= 0 && p < n ? a.sorted[p] : -1;
+  const int v = blockIdx.y * a.lanes + lane;
+  const bool active = v < a.vecs;
+  if ((int)blockIdx.x >= a.spans) {  // zeros of the codes without Gaussians
+    const int64_t c0 = ((int64_t)blockIdx.x - a.spans) * groups * kFillCodes + group;
+    bool none[kFillCodes];
+#pragma unroll
+    for (int k = 0; k < kFillCodes; ++k) {
+      const int64_t c = c0 + (int64_t)k * groups;
+      none[k] = c < a.codes && a.offsets[c] == a.offsets[c + 1];
+    }
+    const float zero[kV] = {};
+#pragma unroll
+    for (int k = 0; k < kFillCodes; ++k)
+      if (none[k] && active)
+        store_vec<TT, kV>(static_cast<TT*>(a.table) + (c0 + (int64_t)k * groups) * a.table_stride + (int64_t)v * kV, zero);
+    return;
   }
-  for (int i = tid; i < len; i += kGradThreads) s_row[i] = a.order[p0 + i];
+  const int none = (int)a.codes;  // places from the first of this code on are without
+  const int64_t p0 = (int64_t)blockIdx.x * a.span;
+  const int pitch = a.part + kPad;
+  for (int i = tid; i < a.span; i += kGradThreads) {
+    const int64_t p = p0 + i;
+    const int at = i + i / a.part * kPad;
+    s_code[at] = p < a.n ? a.sorted[p] : none;
+    s_row[at] = p < a.n ? a.order[p] : 0;
+  }
+  if (tid < 2) {
+    const int64_t p = tid == 0 ? p0 - 1 : p0 + a.span;
+    s_edge[tid] = p >= 0 && p < a.n ? a.sorted[p] : none;
+  }
   if (lane == 0) s_state[group] = 0;
   __syncthreads();
 
-  const int v = blockIdx.y * a.lanes + lane;
-  const bool active = v < a.vecs;
   const TG* rows = static_cast<const TG*>(a.rows) + (int64_t)v * kV;
-  const int q0 = group * a.part, q1 = min(q0 + a.part, len);
+  const int32_t* my_code = s_code + group * pitch;
+  const int32_t* my_row = s_row + group * pitch;
   float acc[kV];
 #pragma unroll
   for (int j = 0; j < kV; ++j) acc[j] = 0.0f;
-  if (q0 < q1) {
-    int cur = s_code[q0 + 1];
-    bool open = s_code[q0] == cur;  // the code began before this part
+  int cur = my_code[0];
+  const bool work = cur != none;
+  if (work) {
+    bool open = (group > 0 ? my_code[a.part - 1 - pitch] : s_edge[0]) == cur;  // the code began before this part
     uint8_t state = 0;
-    for (int q = q0; q < q1; q += kGradRows) {
-      float x[kGradRows][kV];
+    for (int q = 0; q < a.part && cur != none; q += kGradRows) {
+      int code[kGradRows], row[kGradRows];
+#pragma unroll
+      for (int k = 0; k < kGradRows; k += 4) {
+        const int4 c = *reinterpret_cast<const int4*>(my_code + q + k), r = *reinterpret_cast<const int4*>(my_row + q + k);
+        code[k] = c.x, code[k + 1] = c.y, code[k + 2] = c.z, code[k + 3] = c.w;
+        row[k] = r.x, row[k + 1] = r.y, row[k + 2] = r.z, row[k + 3] = r.w;
+      }
+      Raw<TG, kV> x[kGradRows];
 #pragma unroll
       for (int k = 0; k < kGradRows; ++k)
-        if (q + k < q1 && active) load_vec<false, TG, kV>(rows + s_row[q + k] * a.rows_stride, x[k]);
+        if (active && code[k] != none) x[k] = load_raw<false, TG, kV>(rows + row[k] * a.rows_stride);
+      if (code[kGradRows - 1] == cur) {  // in order: all of one code
+#pragma unroll
+        for (int k = 0; k < kGradRows; ++k) {
+          float f[kV];
+          to_floats(x[k], f);
+#pragma unroll
+          for (int j = 0; j < kV; ++j) acc[j] += f[j];
+        }
+        continue;
+      }
 #pragma unroll
       for (int k = 0; k < kGradRows; ++k) {
-        if (q + k < q1) {
-          const int c = s_code[q + k + 1];
-          if (c != cur) {
-            if (open) {
-              state |= kHead;
+        if (code[k] != cur) {
+          if (open) {
+            state |= kHead;
 #pragma unroll
-              for (int j = 0; j < kV; ++j) s_head[j][tid] = acc[j];
-            } else if (active) {
-              write_row<TT, kV>(a, (uint32_t)cur, v, acc);
-            }
-            open = false;
-            cur = c;
-#pragma unroll
-            for (int j = 0; j < kV; ++j) acc[j] = 0.0f;
+            for (int j = 0; j < kV; ++j) s_head[j][tid] = acc[j];
+          } else if (active && cur != none) {
+            write_row<TT, kV>(a, (uint32_t)cur, v, acc);
           }
-          if (active) {
+          open = false;
+          cur = code[k];
 #pragma unroll
-            for (int j = 0; j < kV; ++j) acc[j] += x[k][j];
-          }
+          for (int j = 0; j < kV; ++j) acc[j] = 0.0f;
+        }
+        if (cur != none) {
+          float f[kV];
+          to_floats(x[k], f);
+#pragma unroll
+          for (int j = 0; j < kV; ++j) acc[j] += f[j];
         }
       }
     }
-    if (s_code[q1 + 1] == cur) {  // goes on behind this part
-      state |= open ? kThrough : kTail;
+    if (cur != none) {
+      if ((group + 1 < groups ? my_code[pitch] : s_edge[1]) == cur) {  // goes on behind this part
+        state |= open ? kThrough : kTail;
 #pragma unroll
-      for (int j = 0; j < kV; ++j) s_tail[j][tid] = acc[j];
-    } else if (open) {
-      state |= kHead;
+        for (int j = 0; j < kV; ++j) s_tail[j][tid] = acc[j];
+      } else if (open) {
+        state |= kHead;
 #pragma unroll
-      for (int j = 0; j < kV; ++j) s_head[j][tid] = acc[j];
-    } else if (active) {
-      write_row<TT, kV>(a, (uint32_t)cur, v, acc);
+        for (int j = 0; j < kV; ++j) s_head[j][tid] = acc[j];
+      } else if (active) {
+        write_row<TT, kV>(a, (uint32_t)cur, v, acc);
+      }
     }
     if (lane == 0) s_state[group] = state;
   }
   __syncthreads();
-  if (q0 >= q1 || !active) return;
+  if (!work || !active) return;
   const uint8_t state = s_state[group];
   if (group == 0 && (state & kHead)) {  // the code open at the span's start ends in its first part
     float x[kV];
 #pragma unroll
     for (int j = 0; j < kV; ++j) x[j] = s_head[j][tid];
-    write_partial<kV>(a, blockIdx.x, 0, v, x);
+    store_vec<float, kV>(partial_at<kV>(a, blockIdx.x, 0, v), x);
   }
   // the group where an open code begins (or the span's first) adds its pieces
   if ((state & kTail) || (group == 0 && (state & kThrough))) {
@@ -620,15 +701,39 @@ __global__ void __launch_bounds__(kGradThreads) grad_kernel(const GradArgs a) {
 #pragma unroll
       for (int j = 0; j < kV; ++j) acc[j] += closed ? s_head[j][from] : s_tail[j][from];
     }
-    const bool from_start = (state & kThrough) != 0;
-    if (!closed) write_partial<kV>(a, blockIdx.x, 1, v, acc);
-    else if (from_start) write_partial<kV>(a, blockIdx.x, 0, v, acc);
-    else write_row<TT, kV>(a, (uint32_t)s_code[q1], v, acc);
+    if (closed && !(state & kThrough)) {
+      write_row<TT, kV>(a, (uint32_t)cur, v, acc);
+    } else {
+      store_vec<float, kV>(partial_at<kV>(a, blockIdx.x, closed ? 0 : 1, v), acc);
+    }
   }
 }
 
-// Codes without Gaussians (zeros) and codes over several spans (the sum of
-// their partials, in the order of the spans).
+// Adds the partials of the spans from, from + step, ... of a code whose last span
+// is `last` (where it is the one open at the start).
+template <int kV>
+__device__ __forceinline__ void add_partials(const GradArgs& a, int from, int step, int last, int v,
+                                             float (&acc)[kV]) {
+  constexpr int kAtOnce = 4;
+  for (int s0 = from; s0 <= last; s0 += kAtOnce * step) {
+    Raw<float, kV> x[kAtOnce];
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) {
+      const int s = s0 + k * step;
+      x[k] = load_raw<false, float, kV>(partial_at<kV>(a, min(s, last), s < last ? 1 : 0, v));
+    }
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k)
+      if (s0 + k * step <= last) {
+#pragma unroll
+        for (int j = 0; j < kV; ++j) acc[j] += __uint_as_float(x[k].w[j]);
+      }
+  }
+}
+
+// Codes over several spans: the sum of their partials, in the order of the
+// spans. A group takes a code; codes over many spans are taken by the whole CTA,
+// group g the spans g, g + groups, ..., then a tree over the groups.
 template <typename TT, int kV>
 __global__ void __launch_bounds__(kGradThreads) grad_finish_kernel(const GradArgs a) {
   __shared__ int s_long[kGradThreads];
@@ -640,45 +745,32 @@ __global__ void __launch_bounds__(kGradThreads) grad_finish_kernel(const GradArg
   const int v = blockIdx.y * a.lanes + lane;
   const bool active = v < a.vecs;
   if (tid == 0) s_n_long = 0;
-  __syncthreads();
   const int64_t c = (int64_t)blockIdx.x * groups + group;
+  int first = 0, last = 0;
   if (c < a.codes) {
     const int begin = a.offsets[c], end = a.offsets[c + 1];
-    float acc[kV];
-#pragma unroll
-    for (int j = 0; j < kV; ++j) acc[j] = 0.0f;
-    if (begin == end) {
-      if (active) store_vec<TT, kV>(static_cast<TT*>(a.table) + c * a.table_stride + (int64_t)v * kV, acc);
-    } else {
-      const int first = begin / a.span, last = (end - 1) / a.span;
-      if (last - first >= kLongSpans) {
-        if (lane == 0) s_long[atomicAdd(&s_n_long, 1)] = group;
-      } else if (last > first && active) {
-        for (int s = first; s <= last; ++s) {
-          const float* p = a.partial + ((int64_t)s * 2 + (s < last)) * a.cols + (int64_t)v * kV;
-#pragma unroll
-          for (int j = 0; j < kV; ++j) acc[j] += p[j];
-        }
-        write_row<TT, kV>(a, (uint32_t)c, v, acc);
-      }
-    }
+    if (begin < end) first = begin / a.span, last = (end - 1) / a.span;
   }
-  __syncthreads();
-  for (int k = 0; k < s_n_long; ++k) {  // the order of these codes does not matter
+  const bool is_long = last - first >= kLongSpans;
+  if (__syncthreads_or(is_long)) {
+    if (is_long && lane == 0) s_long[atomicAdd(&s_n_long, 1)] = group;
+    __syncthreads();
+  }
+  float acc[kV];
+#pragma unroll
+  for (int j = 0; j < kV; ++j) acc[j] = 0.0f;
+  if (last > first && !is_long && active) {
+    add_partials<kV>(a, first, 1, last, v, acc);
+    write_row<TT, kV>(a, (uint32_t)c, v, acc);
+  }
+  const int n_long = s_n_long;
+  for (int k = 0; k < n_long; ++k) {  // the order of these codes does not matter
     const int64_t code = (int64_t)blockIdx.x * groups + s_long[k];
     const int begin = a.offsets[code], end = a.offsets[code + 1];
-    const int first = begin / a.span, last = (end - 1) / a.span;
-    float acc[kV];
+    const int from = begin / a.span, to = (end - 1) / a.span;
 #pragma unroll
     for (int j = 0; j < kV; ++j) acc[j] = 0.0f;
-    if (active) {
-#pragma unroll 4
-      for (int s = first + group; s <= last; s += groups) {
-        const float* p = a.partial + ((int64_t)s * 2 + (s < last)) * a.cols + (int64_t)v * kV;
-#pragma unroll
-        for (int j = 0; j < kV; ++j) acc[j] += p[j];
-      }
-    }
+    if (active) add_partials<kV>(a, from + group, groups, to, v, acc);
 #pragma unroll
     for (int j = 0; j < kV; ++j) s_sum[j][tid] = acc[j];
     for (int half = groups / 2; half > 0; half /= 2) {
@@ -734,18 +826,23 @@ int vector_of(int64_t cols, const void* a, int a_size, int64_t a_stride, const v
   return 1;
 }
 
-template <typename TT, typename TR>
-cudaError_t launch_lookup(LookupArgs a, int v, cudaStream_t s) {
+template <typename TI, typename TT, typename TR>
+cudaError_t launch_lookup(const LookupArgs& a, int v, cudaStream_t s) {
   const int64_t per_cta = (int64_t)(kLookupThreads / a.lanes) * kLookupRows;
   const sarr::LaunchShape shape{dim3((unsigned)((a.n + per_cta - 1) / per_cta)), kLookupThreads, 0, false, 1};
   sarr::count_launches(1);
-  if (v == 16 / (int)sizeof(TT)) return sarr::launch(lookup_kernel<TT, TR, 16 / (int)sizeof(TT)>, shape, s, a);
-  if (v == 2) return sarr::launch(lookup_kernel<TT, TR, 2>, shape, s, a);
-  return sarr::launch(lookup_kernel<TT, TR, 1>, shape, s, a);
+  if (v == 16 / (int)sizeof(TR)) return sarr::launch(lookup_kernel<TI, TT, TR, 16 / (int)sizeof(TR)>, shape, s, a);
+  if (v == 2) return sarr::launch(lookup_kernel<TI, TT, TR, 2>, shape, s, a);
+  return sarr::launch(lookup_kernel<TI, TT, TR, 1>, shape, s, a);
+}
+
+template <typename TT, typename TR>
+cudaError_t launch_lookup(const LookupArgs& a, bool wide, int v, cudaStream_t s) {
+  return wide ? launch_lookup<long long, TT, TR>(a, v, s) : launch_lookup<int, TT, TR>(a, v, s);
 }
 
 struct SortPlan {
-  int bits, passes, digit_bits, tiles;
+  int bits, passes, digit_bits, rounds, tiles;
   size_t key_bytes, counts_at, totals_at, bytes;
 };
 
@@ -755,7 +852,11 @@ SortPlan sort_plan(int64_t n, int64_t codes) {
   while (((int64_t)1 << P.bits) <= codes) ++P.bits;  // keys 0 .. codes
   P.passes = (P.bits + kMaxDigitBits - 1) / kMaxDigitBits;
   P.digit_bits = (P.bits + P.passes - 1) / P.passes;
-  P.tiles = (int)((n + kTile - 1) / kTile);
+  const int64_t thousands = (n + kSortThreads - 1) / kSortThreads;
+  const int64_t least = thousands <= kMaxRounds ? thousands : (thousands + kManyTiles - 1) / kManyTiles;
+  P.rounds = 1;
+  while (P.rounds < least && P.rounds < kMaxRounds) P.rounds *= 2;
+  P.tiles = (int)((thousands + P.rounds - 1) / P.rounds);
   P.key_bytes = P.counts_at = P.totals_at = 0;
   P.bytes = 0;  // one tile: shared memory holds it all
   if (P.tiles > 1) {
@@ -770,7 +871,15 @@ SortPlan sort_plan(int64_t n, int64_t codes) {
 
 // The tile kernels use more than 48 KB of shared memory; the permission is per
 // device, asked for once.
-constexpr size_t kTileSmem = sizeof(TileShared);
+template <int kRounds>
+cudaError_t allow_tile_smem() {
+  const cudaError_t e = cudaFuncSetAttribute(sort_tile_kernel<kRounds>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             (int)sizeof(TileShared<kRounds>));
+  if (e != cudaSuccess) return e;
+  return cudaFuncSetAttribute(sort_scatter_kernel<kRounds>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                              (int)(sizeof(TileShared<kRounds>) + 4 * kMaxBins));
+}
+
 cudaError_t allow_sort_smem() {
   static std::atomic<uint64_t> done{0};
   int dev = 0;
@@ -778,24 +887,24 @@ cudaError_t allow_sort_smem() {
   if (e != cudaSuccess) return e;
   const uint64_t bit = dev < 64 ? (uint64_t)1 << dev : 0;
   if (bit & done.load(std::memory_order_acquire)) return cudaSuccess;
-  e = cudaFuncSetAttribute(sort_tile_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kTileSmem);
-  if (e != cudaSuccess) return e;
-  e = cudaFuncSetAttribute(sort_scatter_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           (int)(kTileSmem + 4 * kMaxBins));
-  if (e != cudaSuccess) return e;
+  if ((e = allow_tile_smem<1>()) != cudaSuccess || (e = allow_tile_smem<2>()) != cudaSuccess ||
+      (e = allow_tile_smem<4>()) != cudaSuccess || (e = allow_tile_smem<8>()) != cudaSuccess)
+    return e;
   done.fetch_or(bit, std::memory_order_release);
   return cudaSuccess;
 }
 
+template <int kRounds>
 cudaError_t run_sort(SortArgs a, const SortPlan& P, char* w, int32_t* order, int32_t* sorted, int32_t* offsets,
                      cudaStream_t s) {
+  constexpr size_t kSmem = sizeof(TileShared<kRounds>);
   if (P.tiles <= 1) {
     a.key_out = reinterpret_cast<uint32_t*>(sorted);
     a.place_out = order;
     a.offsets = offsets;
     a.bits = P.bits;
     sarr::count_launches(1);
-    return sarr::launch(sort_tile_kernel, {dim3(1), kSortThreads, kTileSmem, false, 1}, s, a);
+    return sarr::launch(sort_tile_kernel<kRounds>, {dim3(1), kSortThreads, kSmem, false, 1}, s, a);
   }
   a.tiles = P.tiles;
   a.counts = reinterpret_cast<int32_t*>(w + P.counts_at);
@@ -811,13 +920,13 @@ cudaError_t run_sort(SortArgs a, const SortPlan& P, char* w, int32_t* order, int
     a.key_out = key;
     a.place_out = place;
     a.offsets = P.passes == 1 ? offsets : nullptr;
-    const unsigned bins = 1u << a.bits;
+    const unsigned bins = 1u << a.bits, tiles = (unsigned)P.tiles;
     sarr::count_launches(3);
-    e = sarr::launch(sort_histogram_kernel, {dim3((unsigned)P.tiles), kSortThreads, 0, p > 0, 1}, s, a);
+    e = sarr::launch(sort_histogram_kernel<kRounds>, {dim3(tiles), kSortThreads, 0, p > 0, 1}, s, a);
     if (e != cudaSuccess) return e;
     e = sarr::launch(sort_prefix_kernel, {dim3((bins + kPrefixBins - 1) / kPrefixBins), kPrefixThreads, 0, true, 1}, s, a);
     if (e != cudaSuccess) return e;
-    e = sarr::launch(sort_scatter_kernel, {dim3((unsigned)P.tiles), kSortThreads, kTileSmem + 4 * bins, true, 1}, s, a);
+    e = sarr::launch(sort_scatter_kernel<kRounds>, {dim3(tiles), kSortThreads, kSmem + 4 * bins, true, 1}, s, a);
     if (e != cudaSuccess) return e;
     a.key_in = key;
     a.place_in = place;
@@ -844,7 +953,7 @@ GradPlan grad_plan(int64_t n, int64_t cols, int64_t vecs) {
   const int groups = kGradThreads / P.lanes;
   P.part = kGradRows;
   while (P.part < kMaxPart && P.part * 2 * groups <= kMaxSpan &&
-         n / ((int64_t)P.part * 2 * groups) * P.tiles >= 148 * 6)
+         n / ((int64_t)P.part * 2 * groups) * P.tiles >= kGradCtas)
     P.part *= 2;
   P.span = P.part * groups;
   P.spans = (n + P.span - 1) / P.span;
@@ -867,13 +976,12 @@ int check_gradient(int64_t n, int64_t codes, int64_t cols, const void* grad_rows
 
 template <typename TG, typename TT, int kV>
 cudaError_t launch_grad_v(const GradArgs& a, const GradPlan& P, cudaStream_t s) {
-  if (P.spans > 0) {
-    sarr::count_launches(1);
-    const cudaError_t e = sarr::launch(grad_kernel<TG, TT, kV>,
-                                       {dim3((unsigned)P.spans, (unsigned)P.tiles), kGradThreads, 0, true, 1}, s, a);
-    if (e != cudaSuccess) return e;
-  }
   const int groups = kGradThreads / P.lanes;
+  const int64_t fills = ((int64_t)a.codes + groups * kFillCodes - 1) / (groups * kFillCodes);
+  sarr::count_launches(1);
+  const cudaError_t e = sarr::launch(
+      grad_kernel<TG, TT, kV>, {dim3((unsigned)(P.spans + fills), (unsigned)P.tiles), kGradThreads, 0, true, 1}, s, a);
+  if (e != cudaSuccess || P.spans <= 1) return e;  // one span: nothing crosses its border
   sarr::count_launches(1);
   return sarr::launch(grad_finish_kernel<TT, kV>,
                       {dim3((unsigned)((a.codes + groups - 1) / groups), (unsigned)P.tiles), kGradThreads, 0, true, 1},
@@ -901,28 +1009,29 @@ extern "C" int sarr_codebook_lookup(int64_t n, int64_t codes, int64_t cols, cons
   if (!aligned(index, index_bits / 8) || !aligned(table, type_size(table_type)) ||
       !aligned(rows, type_size(rows_type)))
     return SARR_ERR_ARG;
-  const int v = vector_of(cols, table, type_size(table_type), table_stride, rows, type_size(rows_type), rows_stride);
+  const int v = vector_of(cols, rows, type_size(rows_type), rows_stride, table, type_size(table_type), table_stride);
   LookupArgs a;
   memset(&a, 0, sizeof(a));
   a.n = n;
   a.codes = (uint32_t)codes;
   a.vecs = (int)(cols / v);
   a.lanes = pow2_at_least(a.vecs, kLookupThreads);
-  a.wide = index_bits == 64;
   a.scale = scale;
   a.index = index;
   a.table = table;
   a.rows = rows;
-  a.table_stride = table_stride;
-  a.rows_stride = rows_stride;
+  a.table_stride = table_stride * type_size(table_type);
+  a.rows_stride = rows_stride * type_size(rows_type);
+  const bool wide = index_bits == 64;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   cudaError_t e;
-  if (table_type == SARR_F32) e = launch_lookup<float, float>(a, v, s);
+  if (table_type == SARR_F32) e = launch_lookup<float, float>(a, wide, v, s);
   else if (table_type == SARR_BF16)
-    e = rows_type == SARR_F32 ? launch_lookup<__nv_bfloat16, float>(a, v, s)
-                              : launch_lookup<__nv_bfloat16, __nv_bfloat16>(a, v, s);
+    e = rows_type == SARR_F32 ? launch_lookup<__nv_bfloat16, float>(a, wide, v, s)
+                              : launch_lookup<__nv_bfloat16, __nv_bfloat16>(a, wide, v, s);
   else
-    e = rows_type == SARR_F32 ? launch_lookup<__half, float>(a, v, s) : launch_lookup<__half, __half>(a, v, s);
+    e = rows_type == SARR_F32 ? launch_lookup<__half, float>(a, wide, v, s)
+                              : launch_lookup<__half, __half>(a, wide, v, s);
   return cuda_status(e);
 }
 
@@ -951,7 +1060,9 @@ extern "C" int sarr_codebook_sort(int64_t n, int64_t codes, const void* index, i
   a.codes = (uint32_t)codes;
   a.wide = index_bits == 64;
   a.index = index;
-  return cuda_status(run_sort(a, sort_plan(n, codes), static_cast<char*>(ws), order, sorted_codes, offsets, s));
+  const SortPlan P = sort_plan(n, codes);
+  const auto run = P.rounds == 1 ? run_sort<1> : P.rounds == 2 ? run_sort<2> : P.rounds == 4 ? run_sort<4> : run_sort<8>;
+  return cuda_status(run(a, P, static_cast<char*>(ws), order, sorted_codes, offsets, s));
 }
 
 extern "C" int sarr_codebook_grad_workspace_size(int64_t n, int64_t cols, size_t* bytes) {
@@ -981,10 +1092,12 @@ extern "C" int sarr_codebook_grad(int64_t n, int64_t codes, int64_t cols, const 
   const GradPlan P = grad_plan(n, cols, cols / v);
   GradArgs a;
   memset(&a, 0, sizeof(a));
+  a.n = (int)n;
   a.cols = cols;
   a.codes = (uint32_t)codes;
   a.vecs = (int)(cols / v);
   a.lanes = P.lanes;
+  a.spans = (int)P.spans;
   a.part = P.part;
   a.span = P.span;
   a.scale = scale;
