@@ -38,11 +38,12 @@ void count_launches(int k);  // the library's launch counter (sarr_abi.cu)
 
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kVecs = 4;                        // 16-byte loads of a thread for a piece, in flight together
-constexpr int kPieceBytes = kThreads * kVecs * 16;  // of the gradient
-constexpr int kNormCtas = 148 * 8;              // the most CTAs (and partials) of one norm_kernel launch
-constexpr int kClipCtas = 148 * 8, kAdamCtas = 148 * 6;
+// A piece is what a CTA takes at a time: kVecs 16-byte loads of each thread.
+// Grids are a few pieces deep per CTA at the largest sizes, fewer CTAs at others.
+constexpr int kNormThreads = 256, kNormVecs = 4, kNormCtas = 148 * 8;  // kNormCtas: the most partials of a launch
+constexpr int kThreads = 256;                                          // of the clip and Adam kernels
+constexpr int kClipVecs = 2, kClipCtas = 148 * 8;
+constexpr int kAdamVecs = 1, kAdamCtas = 148 * 96;
 constexpr int kSmallList = 16, kMediumList = 96, kLargeList = 512;  // tensors of one launch (kernel parameters)
 constexpr int kAdamRanges = 64;
 
@@ -119,9 +120,9 @@ __device__ __forceinline__ double norm_join(double a, double b) {
 }
 
 // Over the CTA, in a fixed order; every thread gets the result.
-template <bool kInf>
+template <int kCta, bool kInf>
 __device__ __forceinline__ double block_join(double x) {
-  __shared__ double s[kThreads / 32];
+  __shared__ double s[kCta / 32];
   __shared__ double s_all;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) x = norm_join<kInf>(x, __shfl_xor_sync(0xffffffffu, x, o));
@@ -130,23 +131,11 @@ __device__ __forceinline__ double block_join(double x) {
   if (threadIdx.x == 0) {
     double t = s[0];
 #pragma unroll
-    for (int k = 1; k < kThreads / 32; ++k) t = norm_join<kInf>(t, s[k]);
+    for (int k = 1; k < kCta / 32; ++k) t = norm_join<kInf>(t, s[k]);
     s_all = t;
   }
   __syncthreads();
   return s_all;
-}
-
-// The tensor that holds piece `p`.
-template <int kMax>
-__device__ __forceinline__ int find_tensor(const TensorList<kMax>& L, int64_t p) {
-  int lo = 0, hi = L.n - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi) / 2;
-    if (L.e[mid].piece_end > p) hi = mid;
-    else lo = mid + 1;
-  }
-  return lo;
 }
 
 template <int kMax>
@@ -158,15 +147,15 @@ __device__ __forceinline__ int64_t first_piece(const TensorList<kMax>& L, int t)
 // begin or end between 16-byte boundaries) element by element.
 template <int kType, bool kInf>
 __device__ __forceinline__ double piece_norm(const Entry& E, int64_t piece, double acc) {
-  constexpr int kPer = kType == SARR_F32 ? 4 : 8, kElems = kThreads * kVecs * kPer;  // of 16 bytes, of a piece
+  constexpr int kPer = kType == SARR_F32 ? 4 : 8, kElems = kNormThreads * kNormVecs * kPer;  // of 16 bytes, of a piece
   const int64_t at = piece * kElems - E.lead;
   if (at >= 0 && at + kElems <= E.count) {
     const uint4* p = reinterpret_cast<const uint4*>(static_cast<const char*>(E.in) + at * (16 / kPer));
-    uint4 q[kVecs];
+    uint4 q[kNormVecs];
 #pragma unroll
-    for (int k = 0; k < kVecs; ++k) q[k] = p[k * kThreads + threadIdx.x];
+    for (int k = 0; k < kNormVecs; ++k) q[k] = p[k * kNormThreads + threadIdx.x];
 #pragma unroll
-    for (int k = 0; k < kVecs; ++k) {
+    for (int k = 0; k < kNormVecs; ++k) {
       float x[8];
       unpack(q[k], kType, x);
 #pragma unroll
@@ -175,36 +164,28 @@ __device__ __forceinline__ double piece_norm(const Entry& E, int64_t piece, doub
   } else {
     const int64_t end = min(at + kElems, E.count);
 #pragma unroll 4
-    for (int64_t i = max(at, (int64_t)0) + threadIdx.x; i < end; i += kThreads)
+    for (int64_t i = max(at, (int64_t)0) + threadIdx.x; i < end; i += kNormThreads)
       acc = norm_add<kInf>(acc, load_as_float(E.in, kType, i));
   }
   return acc;
 }
 
 template <int kMax, bool kInf>
-__global__ void __launch_bounds__(kThreads, 8) norm_kernel(const __grid_constant__ TensorList<kMax> L,
+__global__ void __launch_bounds__(kNormThreads, 8) norm_kernel(const __grid_constant__ TensorList<kMax> L,
                                                         double* __restrict__ partial) {
   sarr::dependents_may_start();
   sarr::wait_for_previous();
-  const int64_t p0 = L.pieces * blockIdx.x / gridDim.x, p1 = L.pieces * (blockIdx.x + 1) / gridDim.x;
   double acc = 0.0;
-  if (p0 < p1) {
-    int t = find_tensor(L, p0);
-    int64_t first = first_piece(L, t), p = p0;
-    while (p < p1) {
-      const Entry E = L.e[t];
-      const int64_t stop = min(p1, E.piece_end);
-      if (E.type == SARR_F32)
-        for (; p < stop; ++p) acc = piece_norm<SARR_F32, kInf>(E, p - first, acc);
-      else if (E.type == SARR_BF16)
-        for (; p < stop; ++p) acc = piece_norm<SARR_BF16, kInf>(E, p - first, acc);
-      else
-        for (; p < stop; ++p) acc = piece_norm<SARR_F16, kInf>(E, p - first, acc);
-      first = E.piece_end;
-      ++t;
-    }
+  int t = 0;
+  int64_t first = 0, stop = L.e[0].piece_end;
+  for (int64_t p = blockIdx.x; p < L.pieces; p += gridDim.x) {
+    while (p >= stop) first = stop, stop = L.e[++t].piece_end;
+    const Entry& E = L.e[t];
+    if (E.type == SARR_F32) acc = piece_norm<SARR_F32, kInf>(E, p - first, acc);
+    else if (E.type == SARR_BF16) acc = piece_norm<SARR_BF16, kInf>(E, p - first, acc);
+    else acc = piece_norm<SARR_F16, kInf>(E, p - first, acc);
   }
-  acc = block_join<kInf>(acc);
+  acc = block_join<kNormThreads, kInf>(acc);
   if (threadIdx.x == 0) partial[blockIdx.x] = acc;
 }
 
@@ -213,7 +194,7 @@ template <bool kInf>
 __device__ __forceinline__ double total_norm(const double* __restrict__ partial, int n) {
   double acc = 0.0;
   for (int i = threadIdx.x; i < n; i += kThreads) acc = norm_join<kInf>(acc, partial[i]);
-  acc = block_join<kInf>(acc);
+  acc = block_join<kThreads, kInf>(acc);
   return kInf ? acc : sqrt(acc);
 }
 
@@ -261,16 +242,16 @@ __device__ __forceinline__ void store_scaled(char* o, const float* x, int n, flo
 template <int kIn, int kOut>
 __device__ __forceinline__ void piece_clip(const Entry& E, int64_t piece, float c) {
   constexpr int kPer = kIn == SARR_F32 ? 4 : 8, kOutSize = kOut == SARR_F32 ? 4 : 2;
-  constexpr int kElems = kThreads * kVecs * kPer;
+  constexpr int kElems = kThreads * kClipVecs * kPer;
   const int64_t at = piece * kElems - E.lead;
   if (E.vec && at >= 0 && at + kElems <= E.count) {
     const uint4* p = reinterpret_cast<const uint4*>(static_cast<const char*>(E.in) + at * (16 / kPer));
     char* o = static_cast<char*>(E.out) + at * kOutSize;
-    uint4 q[kVecs];
+    uint4 q[kClipVecs];
 #pragma unroll
-    for (int k = 0; k < kVecs; ++k) q[k] = p[k * kThreads + threadIdx.x];
+    for (int k = 0; k < kClipVecs; ++k) q[k] = p[k * kThreads + threadIdx.x];
 #pragma unroll
-    for (int k = 0; k < kVecs; ++k) {
+    for (int k = 0; k < kClipVecs; ++k) {
       float x[8];
       unpack(q[k], kIn, x);
       store_scaled<kOut>(o + (k * kThreads + (int)threadIdx.x) * kPer * kOutSize, x, kPer, c);
@@ -283,11 +264,6 @@ __device__ __forceinline__ void piece_clip(const Entry& E, int64_t piece, float 
   }
 }
 
-template <int kIn, int kOut>
-__device__ __forceinline__ void clip_run(const Entry& E, int64_t from, int64_t to, float c) {
-  for (int64_t p = to - 1; p >= from; --p) piece_clip<kIn, kOut>(E, p, c);
-}
-
 template <int kMax, bool kInf>
 __global__ void __launch_bounds__(kThreads, 8) clip_kernel(const __grid_constant__ TensorList<kMax> L,
                                                         const double* __restrict__ partial, int n_partial,
@@ -296,26 +272,25 @@ __global__ void __launch_bounds__(kThreads, 8) clip_kernel(const __grid_constant
   const double norm = total_norm<kInf>(partial, n_partial);
   if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = (float)norm;
   const float c = clip_coef(norm, max_norm);
-  const int64_t p0 = L.pieces * blockIdx.x / gridDim.x;
-  int64_t p1 = L.pieces * (blockIdx.x + 1) / gridDim.x;
-  if (p0 >= p1) return;
-  for (int t = find_tensor(L, p1 - 1); p1 > p0; --t) {
-    const Entry E = L.e[t];
-    const int64_t first = first_piece(L, t), from = max(p0, first) - first, to = p1 - first;
-    p1 = max(p0, first);
+  int t = L.n - 1;
+  int64_t first = first_piece(L, t);
+  for (int64_t p = L.pieces - 1 - blockIdx.x; p >= 0; p -= gridDim.x) {
+    while (p < first) first = first_piece(L, --t);
+    const Entry& E = L.e[t];
     if (c == 1.0f && E.out == E.in) continue;  // in place and nothing to clip: c x is x
-    if (E.type == SARR_F32) clip_run<SARR_F32, SARR_F32>(E, from, to, c);
-    else if (E.type == SARR_BF16 && E.out_type == SARR_BF16) clip_run<SARR_BF16, SARR_BF16>(E, from, to, c);
-    else if (E.type == SARR_BF16) clip_run<SARR_BF16, SARR_F32>(E, from, to, c);
-    else if (E.out_type == SARR_F16) clip_run<SARR_F16, SARR_F16>(E, from, to, c);
-    else clip_run<SARR_F16, SARR_F32>(E, from, to, c);
+    const int64_t piece = p - first;
+    if (E.type == SARR_F32) piece_clip<SARR_F32, SARR_F32>(E, piece, c);
+    else if (E.type == SARR_BF16 && E.out_type == SARR_BF16) piece_clip<SARR_BF16, SARR_BF16>(E, piece, c);
+    else if (E.type == SARR_BF16) piece_clip<SARR_BF16, SARR_F32>(E, piece, c);
+    else if (E.out_type == SARR_F16) piece_clip<SARR_F16, SARR_F16>(E, piece, c);
+    else piece_clip<SARR_F16, SARR_F32>(E, piece, c);
   }
 }
 
 // ---------------------------------------------------------------------------
 // Adam
 // ---------------------------------------------------------------------------
-constexpr int kAdamVecs = 1, kAdamPiece = kThreads * kAdamVecs * 4;  // elements
+constexpr int kAdamPiece = kThreads * kAdamVecs * 4;  // elements
 
 struct AdamRange {
   int64_t begin, count;  // elements of param / exp_avg / exp_avg_sq
@@ -354,11 +329,8 @@ __global__ void __launch_bounds__(kThreads, 6) adam_kernel(const __grid_constant
   const double norm = total_norm<false>(partial, n_partial);
   if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = (float)norm;
   const float c = clip_coef(norm, max_norm);
-  const int64_t p0 = A.pieces * blockIdx.x / gridDim.x, p1 = A.pieces * (blockIdx.x + 1) / gridDim.x;
-  if (p0 >= p1) return;
-  int t = 0;
-  while (A.r[t].piece_end <= p1 - 1) ++t;
-  for (int64_t p = p1 - 1; p >= p0; --p) {
+  int t = A.n - 1;
+  for (int64_t p = A.pieces - 1 - blockIdx.x; p >= 0; p -= gridDim.x) {
     while (t > 0 && p < A.r[t - 1].piece_end) --t;
     const AdamRange& R = A.r[t];
     const int64_t at = (p - (t > 0 ? A.r[t - 1].piece_end : 0)) * kAdamPiece - R.lead, count = R.count;
@@ -489,7 +461,7 @@ int check_overlap(const ListArgs& a) {
 }
 
 template <int kMax>
-void fill_list(TensorList<kMax>& L, const ListArgs& a, int begin, int end) {
+void fill_list(TensorList<kMax>& L, const ListArgs& a, int begin, int end, int piece_bytes) {
   L.n = 0;
   L.pieces = 0;
   for (int i = begin; i < end; ++i) {
@@ -507,7 +479,7 @@ void fill_list(TensorList<kMax>& L, const ListArgs& a, int begin, int end) {
       E.out_type = (uint8_t)(a.out_types ? a.out_types[i] : a.types[i]);
       E.vec = ((reinterpret_cast<uintptr_t>(E.out) - (uintptr_t)E.lead * type_size(E.out_type)) & 15) == 0;
     }
-    const int64_t piece = kPieceBytes / type_size(E.type);
+    const int64_t piece = piece_bytes / type_size(E.type);
     L.pieces += (E.lead + E.count + piece - 1) / piece;
     E.piece_end = L.pieces;
   }
@@ -517,10 +489,10 @@ template <int kMax, bool kInf>
 cudaError_t norm_group(const ListArgs& a, int begin, int end, bool dependent, double* partial, int* n_partial,
                        cudaStream_t s) {
   TensorList<kMax> L;
-  fill_list(L, a, begin, end);
+  fill_list(L, a, begin, end, kNormThreads * kNormVecs * 16);
   if (L.n == 0) return cudaSuccess;
   const unsigned ctas = (unsigned)ctas_for(L.pieces);
-  const cudaError_t e = sarr::launch(norm_kernel<kMax, kInf>, {dim3(ctas), kThreads, 0, dependent, 1}, s, L,
+  const cudaError_t e = sarr::launch(norm_kernel<kMax, kInf>, {dim3(ctas), kNormThreads, 0, dependent, 1}, s, L,
                                      partial + *n_partial);
   *n_partial += (int)ctas;
   sarr::count_launches(1);
@@ -531,7 +503,7 @@ template <int kMax, bool kInf>
 cudaError_t clip_group(const ListArgs& a, int begin, int end, const double* partial, int n_partial,
                        double max_norm, float* norm_out, cudaStream_t s) {
   TensorList<kMax> L;
-  fill_list(L, a, begin, end);
+  fill_list(L, a, begin, end, kThreads * kClipVecs * 16);
   if (L.n == 0) return cudaSuccess;
   const unsigned ctas = (unsigned)std::min<int64_t>(L.pieces, kClipCtas);
   sarr::count_launches(1);
