@@ -585,11 +585,25 @@ __global__ void __launch_bounds__(kGradThreads, 4) grad_kernel(const GradArgs a)
       const int64_t c = c0 + (int64_t)k * groups;
       none[k] = c < a.codes && a.offsets[c] == a.offsets[c + 1];
     }
-    const float zero[kV] = {};
+    if constexpr (kV * sizeof(TT) >= 16) {  // 16 bytes a lane side by side
+      constexpr int kPer = 16 / (int)sizeof(TT), kSteps = kV / kPer;
+      const int64_t col0 = (int64_t)blockIdx.y * a.lanes * kV + lane * kPer;
 #pragma unroll
-    for (int k = 0; k < kFillCodes; ++k)
-      if (none[k] && active)
-        store_vec<TT, kV>(static_cast<TT*>(a.table) + (c0 + (int64_t)k * groups) * a.table_stride + (int64_t)v * kV, zero);
+      for (int k = 0; k < kFillCodes; ++k) {
+        TT* row = static_cast<TT*>(a.table) + (c0 + (int64_t)k * groups) * a.table_stride;
+#pragma unroll
+        for (int j = 0; j < kSteps; ++j) {
+          const int64_t col = col0 + j * a.lanes * kPer;
+          if (none[k] && col < a.cols) *reinterpret_cast<uint4*>(row + col) = make_uint4(0, 0, 0, 0);
+        }
+      }
+    } else {
+      const float zero[kV] = {};
+#pragma unroll
+      for (int k = 0; k < kFillCodes; ++k)
+        if (none[k] && active)
+          store_vec<TT, kV>(static_cast<TT*>(a.table) + (c0 + (int64_t)k * groups) * a.table_stride + (int64_t)v * kV, zero);
+    }
     return;
   }
   const int none = (int)a.codes;  // places from the first of this code on are without
@@ -620,18 +634,18 @@ __global__ void __launch_bounds__(kGradThreads, 4) grad_kernel(const GradArgs a)
     bool open = (group > 0 ? my_code[a.part - 1 - pitch] : s_edge[0]) == cur;  // the code began before this part
     uint8_t state = 0;
     for (int q = 0; q < a.part && cur != none; q += kGradRows) {
-      int code[kGradRows], row[kGradRows];
+      Raw<TG, kV> x[kGradRows];  // of places without a code too: their rows are there, and not added
 #pragma unroll
       for (int k = 0; k < kGradRows; k += 4) {
-        const int4 c = *reinterpret_cast<const int4*>(my_code + q + k), r = *reinterpret_cast<const int4*>(my_row + q + k);
-        code[k] = c.x, code[k + 1] = c.y, code[k + 2] = c.z, code[k + 3] = c.w;
-        row[k] = r.x, row[k + 1] = r.y, row[k + 2] = r.z, row[k + 3] = r.w;
+        const int4 r = *reinterpret_cast<const int4*>(my_row + q + k);
+        if (active) {
+          x[k] = load_raw<false, TG, kV>(rows + r.x * a.rows_stride);
+          x[k + 1] = load_raw<false, TG, kV>(rows + r.y * a.rows_stride);
+          x[k + 2] = load_raw<false, TG, kV>(rows + r.z * a.rows_stride);
+          x[k + 3] = load_raw<false, TG, kV>(rows + r.w * a.rows_stride);
+        }
       }
-      Raw<TG, kV> x[kGradRows];
-#pragma unroll
-      for (int k = 0; k < kGradRows; ++k)
-        if (active && code[k] != none) x[k] = load_raw<false, TG, kV>(rows + row[k] * a.rows_stride);
-      if (code[kGradRows - 1] == cur) {  // in order: all of one code
+      if (my_code[q + kGradRows - 1] == cur) {  // in order: all of one code
 #pragma unroll
         for (int k = 0; k < kGradRows; ++k) {
           float f[kV];
@@ -643,7 +657,8 @@ __global__ void __launch_bounds__(kGradThreads, 4) grad_kernel(const GradArgs a)
       }
 #pragma unroll
       for (int k = 0; k < kGradRows; ++k) {
-        if (code[k] != cur) {
+        const int c = my_code[q + k];
+        if (c != cur) {
           if (open) {
             state |= kHead;
 #pragma unroll
@@ -652,7 +667,7 @@ __global__ void __launch_bounds__(kGradThreads, 4) grad_kernel(const GradArgs a)
             write_row<TT, kV>(a, (uint32_t)cur, v, acc);
           }
           open = false;
-          cur = code[k];
+          cur = c;
 #pragma unroll
           for (int j = 0; j < kV; ++j) acc[j] = 0.0f;
         }
@@ -732,8 +747,9 @@ __device__ __forceinline__ void add_partials(const GradArgs& a, int from, int st
 }
 
 // Codes over several spans: the sum of their partials, in the order of the
-// spans. A group takes a code; codes over many spans are taken by the whole CTA,
-// group g the spans g, g + groups, ..., then a tree over the groups.
+// spans. Each is found at the border behind the span where it begins; a group
+// takes one, and codes over many spans are taken by the whole CTA, group g the
+// spans g, g + groups, ..., then a tree over the groups.
 template <typename TT, int kV>
 __global__ void __launch_bounds__(kGradThreads) grad_finish_kernel(const GradArgs a) {
   __shared__ int s_long[kGradThreads];
@@ -745,15 +761,16 @@ __global__ void __launch_bounds__(kGradThreads) grad_finish_kernel(const GradArg
   const int v = blockIdx.y * a.lanes + lane;
   const bool active = v < a.vecs;
   if (tid == 0) s_n_long = 0;
-  const int64_t c = (int64_t)blockIdx.x * groups + group;
-  int first = 0, last = 0;
-  if (c < a.codes) {
-    const int begin = a.offsets[c], end = a.offsets[c + 1];
-    if (begin < end) first = begin / a.span, last = (end - 1) / a.span;
+  int first = blockIdx.x * groups + group, last = first, code = (int)a.codes;
+  if (first < a.spans - 1) {
+    const int64_t border = (int64_t)(first + 1) * a.span;
+    code = a.sorted[border - 1];
+    if (code < (int)a.codes && a.sorted[border] == code && a.offsets[code] / a.span == first)
+      last = (a.offsets[code + 1] - 1) / a.span;
   }
   const bool is_long = last - first >= kLongSpans;
   if (__syncthreads_or(is_long)) {
-    if (is_long && lane == 0) s_long[atomicAdd(&s_n_long, 1)] = group;
+    if (is_long && lane == 0) s_long[atomicAdd(&s_n_long, 1)] = code;
     __syncthreads();
   }
   float acc[kV];
@@ -761,16 +778,16 @@ __global__ void __launch_bounds__(kGradThreads) grad_finish_kernel(const GradArg
   for (int j = 0; j < kV; ++j) acc[j] = 0.0f;
   if (last > first && !is_long && active) {
     add_partials<kV>(a, first, 1, last, v, acc);
-    write_row<TT, kV>(a, (uint32_t)c, v, acc);
+    write_row<TT, kV>(a, (uint32_t)code, v, acc);
   }
   const int n_long = s_n_long;
   for (int k = 0; k < n_long; ++k) {  // the order of these codes does not matter
-    const int64_t code = (int64_t)blockIdx.x * groups + s_long[k];
-    const int begin = a.offsets[code], end = a.offsets[code + 1];
-    const int from = begin / a.span, to = (end - 1) / a.span;
+    code = s_long[k];
+    first = a.offsets[code] / a.span;
+    last = (a.offsets[code + 1] - 1) / a.span;
 #pragma unroll
     for (int j = 0; j < kV; ++j) acc[j] = 0.0f;
-    if (active) add_partials<kV>(a, from + group, groups, to, v, acc);
+    if (active) add_partials<kV>(a, first + group, groups, last, v, acc);
 #pragma unroll
     for (int j = 0; j < kV; ++j) s_sum[j][tid] = acc[j];
     for (int half = groups / 2; half > 0; half /= 2) {
@@ -984,7 +1001,7 @@ cudaError_t launch_grad_v(const GradArgs& a, const GradPlan& P, cudaStream_t s) 
   if (e != cudaSuccess || P.spans <= 1) return e;  // one span: nothing crosses its border
   sarr::count_launches(1);
   return sarr::launch(grad_finish_kernel<TT, kV>,
-                      {dim3((unsigned)((a.codes + groups - 1) / groups), (unsigned)P.tiles), kGradThreads, 0, true, 1},
+                      {dim3((unsigned)((P.spans - 1 + groups - 1) / groups), (unsigned)P.tiles), kGradThreads, 0, true, 1},
                       s, a);
 }
 
