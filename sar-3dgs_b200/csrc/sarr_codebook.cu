@@ -203,6 +203,7 @@ constexpr int kMaxRounds = 8;                          // keys per thread
 constexpr int kLocalBits = 9, kLocalBins = 1 << kLocalBits;  // of a pass inside a tile, at most
 constexpr int kMaxDigitBits = 13, kMaxBins = 1 << kMaxDigitBits;
 constexpr int kPrefixThreads = 256, kPrefixBins = 32;  // bins of a CTA; its threads split the tiles 8 ways
+constexpr int kOneTile = 4;                            // up to 4096 keys in one tile
 constexpr int kManyTiles = 148;                        // tiles grow until there are no more of them than SMs
 
 struct SortArgs {
@@ -215,7 +216,7 @@ struct SortArgs {
   uint32_t* key_out;
   int32_t* place_out;
   int32_t *counts, *totals;  // [tiles][bins], [bins]
-  int shift, bits;           // of this pass's digit
+  int shift, bits, bins;     // of this pass's digit; with one pass bins = codes + 1, else 2^bits
   int tiles;
   int32_t* offsets;          // written by the scatter of a sort of one pass, else null
 };
@@ -224,7 +225,7 @@ template <int kRounds>
 struct TileShared {
   uint32_t key[kSortThreads * kRounds];
   int32_t place[kSortThreads * kRounds];
-  uint16_t count[kSortWarps][kLocalBins];
+  uint16_t count[kSortWarps][kLocalBins];  // as many bytes as kMaxBins words
   int32_t digit[kLocalBins];
   int32_t warp_sum[kSortWarps];
 };
@@ -363,8 +364,8 @@ __global__ void __launch_bounds__(kSortThreads) sort_tile_kernel(const SortArgs 
       a.place_out[e] = place[r];
     }
   }
+  if (!a.offsets) return;
   // the first place whose key is >= c
-#pragma unroll 4
   for (int64_t c = threadIdx.x; c <= a.codes; c += kSortThreads) {
     int lo = 0, hi = a.n;
     while (lo < hi) {
@@ -382,7 +383,7 @@ __global__ void __launch_bounds__(kSortThreads) sort_histogram_kernel(const Sort
   __shared__ int32_t s_bin[kMaxBins];
   sarr::dependents_may_start();
   sarr::wait_for_previous();
-  const int bins = 1 << a.bits, tile0 = blockIdx.x * kTile, len = min(kTile, a.n - tile0);
+  const int bins = a.bins, mask = (1 << a.bits) - 1, tile0 = blockIdx.x * kTile, len = min(kTile, a.n - tile0);
   uint32_t key[kRounds];
 #pragma unroll
   for (int r = 0; r < kRounds; ++r) {
@@ -393,7 +394,7 @@ __global__ void __launch_bounds__(kSortThreads) sort_histogram_kernel(const Sort
   __syncthreads();
 #pragma unroll
   for (int r = 0; r < kRounds; ++r)
-    if (r * kSortThreads + threadIdx.x < len) atomicAdd(s_bin + ((key[r] >> a.shift) & (bins - 1)), 1);
+    if (r * kSortThreads + threadIdx.x < len) atomicAdd(s_bin + ((key[r] >> a.shift) & mask), 1);
   __syncthreads();
   for (int d = threadIdx.x; d < bins; d += kSortThreads) a.counts[(int64_t)blockIdx.x * bins + d] = s_bin[d];
 }
@@ -404,7 +405,7 @@ __global__ void __launch_bounds__(kPrefixThreads) sort_prefix_kernel(const SortA
   __shared__ int32_t s_sum[kSplit][kPrefixBins];
   sarr::dependents_may_start();
   sarr::wait_for_previous();
-  const int bins = 1 << a.bits, d = blockIdx.x * kPrefixBins + (threadIdx.x & (kPrefixBins - 1));
+  const int bins = a.bins, d = blockIdx.x * kPrefixBins + (threadIdx.x & (kPrefixBins - 1));
   const int part = threadIdx.x / kPrefixBins, per = (a.tiles + kSplit - 1) / kSplit;
   const int t0 = min(part * per, a.tiles), t1 = min(t0 + per, a.tiles);
   int32_t* c = a.counts + d;
@@ -437,41 +438,41 @@ __global__ void __launch_bounds__(kPrefixThreads) sort_prefix_kernel(const SortA
 }
 
 template <int kRounds>
-__global__ void __launch_bounds__(kSortThreads) sort_scatter_kernel(const SortArgs a) {
-  constexpr int kTile = kSortThreads * kRounds, kBinsEach = kMaxBins / kSortThreads;
+__global__ void __launch_bounds__(kSortThreads, kRounds <= 4 ? 2 : 1) sort_scatter_kernel(const SortArgs a) {
+  constexpr int kTile = kSortThreads * kRounds;
   TileShared<kRounds>& S = *reinterpret_cast<TileShared<kRounds>*>(s_sort);
   int32_t* s_base = reinterpret_cast<int32_t*>(s_sort + sizeof(TileShared<kRounds>));  // [bins]
   uint32_t key[kRounds];
   int32_t place[kRounds];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, begin = warp * kRounds * 32 + lane;
-  const int bins = 1 << a.bits, tile0 = blockIdx.x * kTile, len = min(kTile, a.n - tile0);
+  const int bins = a.bins, mask = (1 << a.bits) - 1, tile0 = blockIdx.x * kTile, len = min(kTile, a.n - tile0);
   sarr::dependents_may_start();
   if (a.key_in) sarr::wait_for_previous();  // the first pass's keys are the caller's
   sort_tile<kRounds>(a, S, key, place, tile0, len, a.shift, a.bits);
   if (!a.key_in) sarr::wait_for_previous();
   // where each digit begins, and in it this tile's keys
   {
-    const int each = max(bins / kSortThreads, 1), first = tid * each;
-    int x[kBinsEach], before[kBinsEach], sum = 0;
-#pragma unroll
-    for (int k = 0; k < kBinsEach; ++k) {
-      const bool have = k < each && first + k < bins;
-      x[k] = have ? __ldcg(a.totals + first + k) : 0;
-      before[k] = have ? __ldcg(a.counts + (int64_t)blockIdx.x * bins + first + k) : 0;
-      sum += x[k];
+    // (the tile's counts are not needed any more: its row of the counts goes there)
+    int32_t* s_before = reinterpret_cast<int32_t*>(S.count);
+    const int32_t* before = a.counts + (int64_t)blockIdx.x * bins;
+#pragma unroll 4
+    for (int d = tid; d < bins; d += kSortThreads) {
+      s_base[d] = __ldcg(a.totals + d);
+      s_before[d] = __ldcg(before + d);
     }
+    __syncthreads();
+    const int each = (bins + kSortThreads - 1) / kSortThreads, first = min(tid * each, bins), end = min(first + each, bins);
+    int sum = 0;
+    for (int d = first; d < end; ++d) sum += s_base[d];
     const int incl = warp_inclusive(sum, lane);
     if (lane == 31) S.warp_sum[warp] = incl;
     __syncthreads();
     int at = incl - sum + warps_before(S.warp_sum, lane, warp);
-#pragma unroll
-    for (int k = 0; k < kBinsEach; ++k) {
-      const int d = first + k;
-      if (k < each && d < bins) {
-        s_base[d] = at + before[k];
-        if (a.offsets && blockIdx.x == 0 && d <= (int)a.codes) a.offsets[d] = at;
-      }
-      at += x[k];
+    for (int d = first; d < end; ++d) {
+      const int x = s_base[d];
+      s_base[d] = at + s_before[d];
+      if (a.offsets && blockIdx.x == 0) a.offsets[d] = at;
+      at += x;
     }
   }
   __syncthreads();
@@ -480,8 +481,8 @@ __global__ void __launch_bounds__(kSortThreads) sort_scatter_kernel(const SortAr
   for (int r = 0; r < kRounds; ++r) {
     const int e = begin + 32 * r;
     if (e < len) {
-      const uint32_t d = (key[r] >> a.shift) & (bins - 1);
-      if (e == 0 || ((S.key[e - 1] >> a.shift) & (bins - 1)) != d) s_base[d] -= e;
+      const uint32_t d = (key[r] >> a.shift) & mask;
+      if (e == 0 || ((S.key[e - 1] >> a.shift) & mask) != d) s_base[d] -= e;
     }
   }
   __syncthreads();
@@ -489,7 +490,7 @@ __global__ void __launch_bounds__(kSortThreads) sort_scatter_kernel(const SortAr
   for (int r = 0; r < kRounds; ++r) {
     const int e = begin + 32 * r;
     if (e < len) {
-      const int to = s_base[(key[r] >> a.shift) & (bins - 1)] + e;
+      const int to = s_base[(key[r] >> a.shift) & mask] + e;
       a.key_out[to] = key[r];
       a.place_out[to] = place[r];
     }
@@ -561,7 +562,7 @@ __device__ __forceinline__ float* partial_at(const GradArgs& a, int span, int sl
 }
 
 template <typename TG, typename TT, int kV>
-__global__ void __launch_bounds__(kGradThreads, 4) grad_kernel(const GradArgs a) {
+__global__ void __launch_bounds__(kGradThreads, kV >= 8 ? 3 : 4) grad_kernel(const GradArgs a) {
   // codes and rows of the parts, each part kPad words behind the one before, so
   // that groups at the same place of their parts use different banks
   constexpr int kPad = 4, kWords = kMaxSpan + kMaxSpan / kGradRows * kPad;
@@ -870,7 +871,7 @@ SortPlan sort_plan(int64_t n, int64_t codes) {
   P.passes = (P.bits + kMaxDigitBits - 1) / kMaxDigitBits;
   P.digit_bits = (P.bits + P.passes - 1) / P.passes;
   const int64_t thousands = (n + kSortThreads - 1) / kSortThreads;
-  const int64_t least = thousands <= kMaxRounds ? thousands : (thousands + kManyTiles - 1) / kManyTiles;
+  const int64_t least = thousands <= kOneTile ? thousands : (thousands + kManyTiles - 1) / kManyTiles;
   P.rounds = 1;
   while (P.rounds < least && P.rounds < kMaxRounds) P.rounds *= 2;
   P.tiles = (int)((thousands + P.rounds - 1) / P.rounds);
@@ -911,6 +912,12 @@ cudaError_t allow_sort_smem() {
   return cudaSuccess;
 }
 
+cudaError_t launch_offsets(const SortArgs& a, const int32_t* sorted, int32_t* offsets, cudaStream_t s) {
+  sarr::count_launches(1);
+  return sarr::launch(sort_offsets_kernel, {dim3((unsigned)(((int64_t)a.codes + 256) / 256)), 256, 0, true, 1}, s, a.n,
+                      a.codes, sorted, offsets);
+}
+
 template <int kRounds>
 cudaError_t run_sort(SortArgs a, const SortPlan& P, char* w, int32_t* order, int32_t* sorted, int32_t* offsets,
                      cudaStream_t s) {
@@ -918,10 +925,11 @@ cudaError_t run_sort(SortArgs a, const SortPlan& P, char* w, int32_t* order, int
   if (P.tiles <= 1) {
     a.key_out = reinterpret_cast<uint32_t*>(sorted);
     a.place_out = order;
-    a.offsets = offsets;
+    a.offsets = P.passes == 1 ? offsets : nullptr;  // more codes than one CTA finds quickly: below
     a.bits = P.bits;
     sarr::count_launches(1);
-    return sarr::launch(sort_tile_kernel<kRounds>, {dim3(1), kSortThreads, kSmem, false, 1}, s, a);
+    const cudaError_t e = sarr::launch(sort_tile_kernel<kRounds>, {dim3(1), kSortThreads, kSmem, false, 1}, s, a);
+    return e != cudaSuccess || P.passes == 1 ? e : launch_offsets(a, sorted, offsets, s);
   }
   a.tiles = P.tiles;
   a.counts = reinterpret_cast<int32_t*>(w + P.counts_at);
@@ -937,7 +945,8 @@ cudaError_t run_sort(SortArgs a, const SortPlan& P, char* w, int32_t* order, int
     a.key_out = key;
     a.place_out = place;
     a.offsets = P.passes == 1 ? offsets : nullptr;
-    const unsigned bins = 1u << a.bits, tiles = (unsigned)P.tiles;
+    a.bins = P.passes == 1 ? (int)a.codes + 1 : 1 << a.bits;
+    const unsigned bins = (unsigned)a.bins, tiles = (unsigned)P.tiles;
     sarr::count_launches(3);
     e = sarr::launch(sort_histogram_kernel<kRounds>, {dim3(tiles), kSortThreads, 0, p > 0, 1}, s, a);
     if (e != cudaSuccess) return e;
@@ -948,10 +957,7 @@ cudaError_t run_sort(SortArgs a, const SortPlan& P, char* w, int32_t* order, int
     a.key_in = key;
     a.place_in = place;
   }
-  if (P.passes == 1) return cudaSuccess;
-  sarr::count_launches(1);
-  return sarr::launch(sort_offsets_kernel, {dim3((unsigned)(((int64_t)a.codes + 256) / 256)), 256, 0, true, 1}, s, a.n,
-                      a.codes, sorted, offsets);
+  return P.passes == 1 ? cudaSuccess : launch_offsets(a, sorted, offsets, s);
 }
 
 struct GradPlan {
