@@ -181,17 +181,18 @@ __global__ void __launch_bounds__(kLookupThreads) lookup_kernel(const LookupArgs
 // sort
 // ---------------------------------------------------------------------------
 // A stable sort of the keys (the codes, `codes` for none). The unit is a tile of
-// 1024 to 8192 keys that one CTA sorts in registers and shared memory: each warp
-// holds a contiguous part of the tile, 32 keys a round; a key's rank among the
-// warp's keys of its digit is a running count plus the lower lanes that vote for
-// the same digit (one vote per bit, so a digit costs the same whatever the keys
-// are), and a scan over the warps' counts and the digits gives every rank its
-// place. Counts are 16 bits wide, two digits to a word.
+// 1024 to 8192 keys that one CTA sorts in registers and shared memory, as words
+// digit << 13 | place in the tile: each warp holds a contiguous part of the tile,
+// 32 words a round; a word's rank among the warp's words of its digit is a running
+// count plus the lower lanes that vote for the same digit (one vote per bit, so a
+// digit costs the same whatever the keys are), and a scan over the warps' counts
+// and the digits gives every rank its place. Counts are 16 bits wide, two digits
+// to a word.
 //
 // One tile: one CTA sorts by every digit and finds the offsets (sort_tile_kernel).
 //
 // More: passes over digits of up to 13 bits (so one pass up to 8191 codes), of
-// three kernels each, which the scheduler may overlap:
+// three kernels each, which overlap (their CTAs fit on an SM together):
 //   histogram  each tile's count of every digit, [tiles][bins]
 //   prefix     per digit the counts of the earlier tiles, and the total
 //   scatter    the tile sorted by the digit, written out behind the smaller digits
@@ -199,12 +200,15 @@ __global__ void __launch_bounds__(kLookupThreads) lookup_kernel(const LookupArgs
 //              first pass sorts its tile before it waits for the other two.
 // With one pass the scan over the totals is the offsets.
 constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32;
-constexpr int kMaxRounds = 8;                          // keys per thread
+constexpr int kMaxRounds = 8;                          // words per thread
+constexpr int kPlaceBits = 13;                         // of a place in a tile
 constexpr int kLocalBits = 9, kLocalBins = 1 << kLocalBits;  // of a pass inside a tile, at most
 constexpr int kMaxDigitBits = 13, kMaxBins = 1 << kMaxDigitBits;
+constexpr int kWholeBits = 32 - kPlaceBits;            // of a key that fits a word
+constexpr int kOneTile = 4;                            // up to 4096 such keys in one tile
 constexpr int kPrefixThreads = 256, kPrefixBins = 32;  // bins of a CTA; its threads split the tiles 8 ways
-constexpr int kOneTile = 4;                            // up to 4096 keys in one tile
 constexpr int kManyTiles = 148;                        // tiles grow until there are no more of them than SMs
+static_assert(kSortThreads * kMaxRounds <= 1 << kPlaceBits, "a place fits its bits");
 
 struct SortArgs {
   int n;
@@ -218,13 +222,20 @@ struct SortArgs {
   int32_t *counts, *totals;  // [tiles][bins], [bins]
   int shift, bits, bins;     // of this pass's digit; with one pass bins = codes + 1, else 2^bits
   int tiles;
+  bool whole;                // words hold the whole key (of up to 19 bits), else the digit
   int32_t* offsets;          // written by the scatter of a sort of one pass, else null
 };
 
+__device__ __forceinline__ uint32_t sort_key(const SortArgs& a, int i) {
+  return a.key_in ? a.key_in[i] : code_of(a.index, a.wide, i, a.codes);
+}
+
+// Where the pass's digit is in a word.
+__device__ __forceinline__ int digit_shift(const SortArgs& a) { return kPlaceBits + (a.whole ? a.shift : 0); }
+
 template <int kRounds>
 struct TileShared {
-  uint32_t key[kSortThreads * kRounds];
-  int32_t place[kSortThreads * kRounds];
+  uint32_t word[kSortThreads * kRounds];
   uint16_t count[kSortWarps][kLocalBins];  // as many bytes as kMaxBins words
   int32_t digit[kLocalBins];
   int32_t warp_sum[kSortWarps];
@@ -244,12 +255,12 @@ __device__ __forceinline__ int warps_before(const int32_t* warp_sum, int lane, i
   return __reduce_add_sync(0xffffffffu, lane < warp ? warp_sum[lane] : 0);
 }
 
-// One stable pass over the tile's keys, which the threads hold: element
-// (warp * kRounds + r) * 32 + lane in key[r]; elements from len on are none. On
+// One stable pass over the tile's words, which the threads hold: element
+// (warp * kRounds + r) * 32 + lane in word[r]; elements from len on are none. On
 // return S holds the tile in order and so do the threads.
 template <int kRounds>
-__device__ __forceinline__ void tile_pass(TileShared<kRounds>& S, uint32_t (&key)[kRounds], int32_t (&place)[kRounds],
-                                          int len, int shift, int bits) {
+__device__ __forceinline__ void tile_pass(TileShared<kRounds>& S, uint32_t (&word)[kRounds], int len, int shift,
+                                          int bits) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, bins = 1 << bits;
   const int first = warp * kRounds * 32 + lane;
   uint16_t* count = S.count[warp];
@@ -257,10 +268,11 @@ __device__ __forceinline__ void tile_pass(TileShared<kRounds>& S, uint32_t (&key
   uint32_t peers[kRounds];
 #pragma unroll
   for (int r = 0; r < kRounds; ++r) peers[r] = __ballot_sync(0xffffffffu, first + 32 * r < len);
-  for (int b = 0; b < bits; ++b) {
+  uint32_t bit = 1u << shift;
+  for (int b = 0; b < bits; ++b, bit += bit) {
 #pragma unroll
     for (int r = 0; r < kRounds; ++r) {
-      const bool one = (key[r] >> (shift + b)) & 1;
+      const bool one = (word[r] & bit) != 0;
       const uint32_t ones = __ballot_sync(0xffffffffu, one);
       peers[r] &= one ? ones : ~ones;
     }
@@ -269,7 +281,7 @@ __device__ __forceinline__ void tile_pass(TileShared<kRounds>& S, uint32_t (&key
   int rank[kRounds];
 #pragma unroll
   for (int r = 0; r < kRounds; ++r) {
-    const uint32_t digit = (key[r] >> shift) & (bins - 1), below = peers[r] & ((1u << lane) - 1);
+    const uint32_t digit = (word[r] >> shift) & (bins - 1), below = peers[r] & ((1u << lane) - 1);
     const bool have = first + 32 * r < len;
     const int before = have ? count[digit] : 0;
     __syncwarp();
@@ -310,40 +322,33 @@ __device__ __forceinline__ void tile_pass(TileShared<kRounds>& S, uint32_t (&key
 #pragma unroll
   for (int r = 0; r < kRounds; ++r) {
     if (first + 32 * r < len) {
-      const uint32_t digit = (key[r] >> shift) & (bins - 1);
-      const int to = S.digit[digit] + count[digit] + rank[r];
-      S.key[to] = key[r];
-      S.place[to] = place[r];
+      const uint32_t digit = (word[r] >> shift) & (bins - 1);
+      S.word[S.digit[digit] + count[digit] + rank[r]] = word[r];
     }
   }
   __syncthreads();
 #pragma unroll
-  for (int r = 0; r < kRounds; ++r) {
-    if (first + 32 * r < len) {
-      key[r] = S.key[first + 32 * r];
-      place[r] = S.place[first + 32 * r];
-    }
-  }
+  for (int r = 0; r < kRounds; ++r)
+    if (first + 32 * r < len) word[r] = S.word[first + 32 * r];
 }
 
-// The tile's keys into the threads, then sorted by `bits` bits from `shift`.
+// The tile's words into the threads, then sorted by the `bits` bits of the digit.
 template <int kRounds>
-__device__ __forceinline__ void sort_tile(const SortArgs& a, TileShared<kRounds>& S, uint32_t (&key)[kRounds],
-                                          int32_t (&place)[kRounds], int tile0, int len, int shift, int bits) {
+__device__ __forceinline__ void sort_tile(const SortArgs& a, TileShared<kRounds>& S, uint32_t (&word)[kRounds],
+                                          int tile0, int len) {
   const int first = (threadIdx.x >> 5) * kRounds * 32 + (threadIdx.x & 31);
 #pragma unroll
   for (int r = 0; r < kRounds; ++r) {
-    const int e = first + 32 * r, i = tile0 + e;
-    key[r] = 0;
-    place[r] = 0;
-    if (e < len) {
-      key[r] = a.key_in ? __ldcg(a.key_in + i) : code_of(a.index, a.wide, i, a.codes);
-      place[r] = a.key_in ? __ldcg(a.place_in + i) : i;
-    }
+    const int e = first + 32 * r;
+    word[r] = e < len ? sort_key(a, tile0 + e) : 0;
   }
-  const int passes = (bits + kLocalBits - 1) / kLocalBits, each = (bits + passes - 1) / passes;
+#pragma unroll
+  for (int r = 0; r < kRounds; ++r)
+    word[r] = (a.whole ? word[r] : (word[r] >> a.shift) & ((1u << a.bits) - 1)) << kPlaceBits | (first + 32 * r);
+  const int passes = (a.bits + kLocalBits - 1) / kLocalBits, each = (a.bits + passes - 1) / passes;
 #pragma unroll 1
-  for (int p = 0; p < passes; ++p) tile_pass<kRounds>(S, key, place, len, shift + p * each, min(each, bits - p * each));
+  for (int p = 0; p < passes; ++p)
+    tile_pass<kRounds>(S, word, len, digit_shift(a) + p * each, min(each, a.bits - p * each));
 }
 
 extern __shared__ __align__(16) unsigned char s_sort[];
@@ -351,17 +356,16 @@ extern __shared__ __align__(16) unsigned char s_sort[];
 template <int kRounds>
 __global__ void __launch_bounds__(kSortThreads) sort_tile_kernel(const SortArgs a) {
   TileShared<kRounds>& S = *reinterpret_cast<TileShared<kRounds>*>(s_sort);
-  uint32_t key[kRounds];
-  int32_t place[kRounds];
+  uint32_t word[kRounds];
   sarr::dependents_may_start();
-  sort_tile<kRounds>(a, S, key, place, 0, a.n, 0, a.bits);
+  sort_tile<kRounds>(a, S, word, 0, a.n);
   const int first = (threadIdx.x >> 5) * kRounds * 32 + (threadIdx.x & 31);
 #pragma unroll
   for (int r = 0; r < kRounds; ++r) {
     const int e = first + 32 * r;
     if (e < a.n) {
-      a.key_out[e] = key[r];
-      a.place_out[e] = place[r];
+      a.key_out[e] = word[r] >> kPlaceBits;
+      a.place_out[e] = word[r] & ((1 << kPlaceBits) - 1);
     }
   }
   if (!a.offsets) return;
@@ -370,37 +374,43 @@ __global__ void __launch_bounds__(kSortThreads) sort_tile_kernel(const SortArgs 
     int lo = 0, hi = a.n;
     while (lo < hi) {
       const int mid = (lo + hi) >> 1;
-      if (S.key[mid] < (uint32_t)c) lo = mid + 1;
+      if (S.word[mid] >> kPlaceBits < (uint32_t)c) lo = mid + 1;
       else hi = mid;
     }
     a.offsets[c] = lo;
   }
 }
 
+// Threads of the histogram: few enough for its CTA beside the other two kernels'.
 template <int kRounds>
-__global__ void __launch_bounds__(kSortThreads) sort_histogram_kernel(const SortArgs a) {
-  constexpr int kTile = kSortThreads * kRounds;
+constexpr int kCountThreads = kRounds >= 8 ? 512 : 256;
+
+template <int kRounds>
+__global__ void __launch_bounds__(kCountThreads<kRounds>, 2048 / kCountThreads<kRounds>)
+    sort_histogram_kernel(const SortArgs a) {
+  constexpr int kTile = kSortThreads * kRounds, kThreads = kCountThreads<kRounds>, kBatch = 4;
   __shared__ int32_t s_bin[kMaxBins];
   sarr::dependents_may_start();
   sarr::wait_for_previous();
   const int bins = a.bins, mask = (1 << a.bits) - 1, tile0 = blockIdx.x * kTile, len = min(kTile, a.n - tile0);
-  uint32_t key[kRounds];
+  for (int d = threadIdx.x; d < bins; d += kThreads) s_bin[d] = 0;
+  __syncthreads();
+#pragma unroll 2
+  for (int e0 = threadIdx.x; e0 < len; e0 += kBatch * kThreads) {
+    uint32_t key[kBatch];
 #pragma unroll
-  for (int r = 0; r < kRounds; ++r) {
-    const int e = r * kSortThreads + threadIdx.x;
-    if (e < len) key[r] = a.key_in ? __ldcg(a.key_in + tile0 + e) : code_of(a.index, a.wide, tile0 + e, a.codes);
+    for (int k = 0; k < kBatch; ++k)
+      if (e0 + k * kThreads < len) key[k] = sort_key(a, tile0 + e0 + k * kThreads);
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k)
+      if (e0 + k * kThreads < len) atomicAdd(s_bin + ((key[k] >> a.shift) & mask), 1);
   }
-  for (int d = threadIdx.x; d < bins; d += kSortThreads) s_bin[d] = 0;
   __syncthreads();
-#pragma unroll
-  for (int r = 0; r < kRounds; ++r)
-    if (r * kSortThreads + threadIdx.x < len) atomicAdd(s_bin + ((key[r] >> a.shift) & mask), 1);
-  __syncthreads();
-  for (int d = threadIdx.x; d < bins; d += kSortThreads) a.counts[(int64_t)blockIdx.x * bins + d] = s_bin[d];
+  for (int d = threadIdx.x; d < bins; d += kThreads) a.counts[(int64_t)blockIdx.x * bins + d] = s_bin[d];
 }
 
 // counts[t][d] becomes the sum of counts[0 .. t-1][d], totals[d] the sum of all.
-__global__ void __launch_bounds__(kPrefixThreads) sort_prefix_kernel(const SortArgs a) {
+__global__ void __launch_bounds__(kPrefixThreads, 8) sort_prefix_kernel(const SortArgs a) {
   constexpr int kSplit = kPrefixThreads / kPrefixBins;
   __shared__ int32_t s_sum[kSplit][kPrefixBins];
   sarr::dependents_may_start();
@@ -411,7 +421,7 @@ __global__ void __launch_bounds__(kPrefixThreads) sort_prefix_kernel(const SortA
   int32_t* c = a.counts + d;
   int sum = 0;
   if (d < bins) {
-#pragma unroll 16
+#pragma unroll 8
     for (int t = t0; t < t1; ++t) sum += __ldcg(c + (int64_t)t * bins);
   }
   s_sum[part][threadIdx.x & (kPrefixBins - 1)] = sum;
@@ -425,12 +435,12 @@ __global__ void __launch_bounds__(kPrefixThreads) sort_prefix_kernel(const SortA
     all += x;
   }
   if (part == 0) a.totals[d] = all;
-  for (int t = t0; t < t1; t += 16) {
-    int x[16];
+  for (int t = t0; t < t1; t += 8) {
+    int x[8];
 #pragma unroll
-    for (int k = 0; k < 16; ++k) x[k] = t + k < t1 ? __ldcg(c + (int64_t)(t + k) * bins) : 0;
+    for (int k = 0; k < 8; ++k) x[k] = t + k < t1 ? __ldcg(c + (int64_t)(t + k) * bins) : 0;
 #pragma unroll
-    for (int k = 0; k < 16; ++k) {
+    for (int k = 0; k < 8; ++k) {
       if (t + k < t1) c[(int64_t)(t + k) * bins] = at;
       at += x[k];
     }
@@ -438,17 +448,17 @@ __global__ void __launch_bounds__(kPrefixThreads) sort_prefix_kernel(const SortA
 }
 
 template <int kRounds>
-__global__ void __launch_bounds__(kSortThreads, kRounds <= 4 ? 2 : 1) sort_scatter_kernel(const SortArgs a) {
+__global__ void __maxnreg__(kRounds <= 4 ? 32 : 40) sort_scatter_kernel(const SortArgs a) {
   constexpr int kTile = kSortThreads * kRounds;
   TileShared<kRounds>& S = *reinterpret_cast<TileShared<kRounds>*>(s_sort);
   int32_t* s_base = reinterpret_cast<int32_t*>(s_sort + sizeof(TileShared<kRounds>));  // [bins]
-  uint32_t key[kRounds];
-  int32_t place[kRounds];
+  uint32_t word[kRounds];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, begin = warp * kRounds * 32 + lane;
-  const int bins = a.bins, mask = (1 << a.bits) - 1, tile0 = blockIdx.x * kTile, len = min(kTile, a.n - tile0);
+  const int bins = a.bins, tile0 = blockIdx.x * kTile, len = min(kTile, a.n - tile0);
+  const int shift = digit_shift(a), mask = (1 << a.bits) - 1;
   sarr::dependents_may_start();
   if (a.key_in) sarr::wait_for_previous();  // the first pass's keys are the caller's
-  sort_tile<kRounds>(a, S, key, place, tile0, len, a.shift, a.bits);
+  sort_tile<kRounds>(a, S, word, tile0, len);
   if (!a.key_in) sarr::wait_for_previous();
   // where each digit begins, and in it this tile's keys
   {
@@ -481,8 +491,8 @@ __global__ void __launch_bounds__(kSortThreads, kRounds <= 4 ? 2 : 1) sort_scatt
   for (int r = 0; r < kRounds; ++r) {
     const int e = begin + 32 * r;
     if (e < len) {
-      const uint32_t d = (key[r] >> a.shift) & mask;
-      if (e == 0 || ((S.key[e - 1] >> a.shift) & mask) != d) s_base[d] -= e;
+      const uint32_t d = (word[r] >> shift) & mask;
+      if (e == 0 || ((S.word[e - 1] >> shift) & mask) != d) s_base[d] -= e;
     }
   }
   __syncthreads();
@@ -490,9 +500,9 @@ __global__ void __launch_bounds__(kSortThreads, kRounds <= 4 ? 2 : 1) sort_scatt
   for (int r = 0; r < kRounds; ++r) {
     const int e = begin + 32 * r;
     if (e < len) {
-      const int to = s_base[(key[r] >> a.shift) & mask] + e;
-      a.key_out[to] = key[r];
-      a.place_out[to] = place[r];
+      const int from = tile0 + (int)(word[r] & ((1 << kPlaceBits) - 1)), to = s_base[(word[r] >> shift) & mask] + e;
+      a.key_out[to] = a.whole ? word[r] >> kPlaceBits : sort_key(a, from);
+      a.place_out[to] = a.key_in ? a.place_in[from] : from;
     }
   }
 }
@@ -861,6 +871,7 @@ cudaError_t launch_lookup(const LookupArgs& a, bool wide, int v, cudaStream_t s)
 
 struct SortPlan {
   int bits, passes, digit_bits, rounds, tiles;
+  bool one;  // one tile sorts it
   size_t key_bytes, counts_at, totals_at, bytes;
 };
 
@@ -871,13 +882,15 @@ SortPlan sort_plan(int64_t n, int64_t codes) {
   P.passes = (P.bits + kMaxDigitBits - 1) / kMaxDigitBits;
   P.digit_bits = (P.bits + P.passes - 1) / P.passes;
   const int64_t thousands = (n + kSortThreads - 1) / kSortThreads;
-  const int64_t least = thousands <= kOneTile ? thousands : (thousands + kManyTiles - 1) / kManyTiles;
+  const bool one = thousands <= kOneTile && P.bits <= kWholeBits;
+  const int64_t least = one ? thousands : (thousands + kManyTiles - 1) / kManyTiles;
   P.rounds = 1;
   while (P.rounds < least && P.rounds < kMaxRounds) P.rounds *= 2;
   P.tiles = (int)((thousands + P.rounds - 1) / P.rounds);
   P.key_bytes = P.counts_at = P.totals_at = 0;
   P.bytes = 0;  // one tile: shared memory holds it all
-  if (P.tiles > 1) {
+  P.one = one || n == 0;
+  if (!P.one) {
     P.key_bytes = round256((size_t)n * 4);
     const int buffers = std::min(P.passes - 1, 2);
     P.counts_at = (size_t)buffers * 2 * P.key_bytes;
@@ -922,7 +935,8 @@ template <int kRounds>
 cudaError_t run_sort(SortArgs a, const SortPlan& P, char* w, int32_t* order, int32_t* sorted, int32_t* offsets,
                      cudaStream_t s) {
   constexpr size_t kSmem = sizeof(TileShared<kRounds>);
-  if (P.tiles <= 1) {
+  a.whole = P.bits <= kWholeBits;
+  if (P.one) {
     a.key_out = reinterpret_cast<uint32_t*>(sorted);
     a.place_out = order;
     a.offsets = P.passes == 1 ? offsets : nullptr;  // more codes than one CTA finds quickly: below
@@ -948,7 +962,7 @@ cudaError_t run_sort(SortArgs a, const SortPlan& P, char* w, int32_t* order, int
     a.bins = P.passes == 1 ? (int)a.codes + 1 : 1 << a.bits;
     const unsigned bins = (unsigned)a.bins, tiles = (unsigned)P.tiles;
     sarr::count_launches(3);
-    e = sarr::launch(sort_histogram_kernel<kRounds>, {dim3(tiles), kSortThreads, 0, p > 0, 1}, s, a);
+    e = sarr::launch(sort_histogram_kernel<kRounds>, {dim3(tiles), (unsigned)kCountThreads<kRounds>, 0, p > 0, 1}, s, a);
     if (e != cudaSuccess) return e;
     e = sarr::launch(sort_prefix_kernel, {dim3((bins + kPrefixBins - 1) / kPrefixBins), kPrefixThreads, 0, true, 1}, s, a);
     if (e != cudaSuccess) return e;
