@@ -247,7 +247,7 @@ int sarr_codebook_sort(int64_t n, int64_t codes, const void *index, int index_bi
  *   elements >= cols. Sums are kept in 32 bits and rounded once, in an order
  *   that depends on the sizes and the codes only, so the result is reproducible.
  *   order, sorted_codes and offsets must be what sarr_codebook_sort wrote for
- *   the same n and codes.
+ *   the same n and codes; order and sorted_codes 16-byte aligned.
  */
 int sarr_codebook_grad_workspace_size(int64_t n, int64_t cols, size_t *bytes);
 int sarr_codebook_grad(int64_t n, int64_t codes, int64_t cols, const void *grad_rows, int rows_type,

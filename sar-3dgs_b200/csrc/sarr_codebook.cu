@@ -129,8 +129,8 @@ __device__ __forceinline__ uint32_t code_of(const void* index, bool wide, int64_
 // ---------------------------------------------------------------------------
 // lookup
 // ---------------------------------------------------------------------------
-constexpr int kLookupThreads = 256;
-constexpr int kLookupRows = 8;  // rows per thread, their loads in flight together
+constexpr int kLookupThreads = 64;
+constexpr int kLookupRows = 6;  // rows per thread, their loads in flight together
 
 struct LookupArgs {
   int64_t n;
@@ -148,7 +148,7 @@ template <typename TI, typename TT, typename TR, int kV>
 __global__ void __launch_bounds__(kLookupThreads) lookup_kernel(const LookupArgs a) {
   const int lane = threadIdx.x & (a.lanes - 1), at_once = kLookupThreads / a.lanes;
   const int64_t i0 = (int64_t)blockIdx.x * at_once * kLookupRows + threadIdx.x / a.lanes;
-  const int64_t left = a.n - i0;  // row k is there where k * at_once < left
+  const int left = (int)min(a.n - i0, (int64_t)kLookupRows * at_once);  // row k is there where k * at_once < left
   const TI* index = static_cast<const TI*>(a.index) + i0;
   uint32_t code[kLookupRows];
 #pragma unroll
@@ -159,19 +159,18 @@ __global__ void __launch_bounds__(kLookupThreads) lookup_kernel(const LookupArgs
     char* to = static_cast<char*>(a.rows) + i0 * a.rows_stride + v * (kV * (int)sizeof(TR));
     Raw<TT, kV> raw[kLookupRows];
 #pragma unroll
-    for (int k = 0; k < kLookupRows; ++k)
+    for (int k = 0; k < kLookupRows; ++k) {
+#pragma unroll
+      for (int j = 0; j < Raw<TT, kV>::kWords; ++j) raw[k].w[j] = 0;
       if (code[k] < a.codes) raw[k] = load_raw<true, TT, kV>(reinterpret_cast<const TT*>(from + code[k] * a.table_stride));
+    }
 #pragma unroll
     for (int k = 0; k < kLookupRows; ++k, to += step) {
+      const float scale = code[k] < a.codes ? a.scale : 0.0f;  // zeros whatever the scale is
       float x[kV];
-      if (code[k] < a.codes) {
-        to_floats(raw[k], x);
+      to_floats(raw[k], x);
 #pragma unroll
-        for (int j = 0; j < kV; ++j) x[j] *= a.scale;
-      } else {  // a row without a code is zeros whatever the scale
-#pragma unroll
-        for (int j = 0; j < kV; ++j) x[j] = 0.0f;
-      }
+      for (int j = 0; j < kV; ++j) x[j] *= scale;
       if (k * at_once < left) store_vec<TR, kV>(reinterpret_cast<TR*>(to), x);
     }
   }
@@ -536,9 +535,10 @@ __global__ void __launch_bounds__(256) sort_offsets_kernel(int n, uint32_t codes
 // the others wait for their rows.
 constexpr int kGradThreads = 256;
 constexpr int kGradRows = 8;     // rows of a group loaded together
-constexpr int kMaxPart = 64;     // places of a group, at most
+constexpr int kMaxPart = 64;     // places of a group, at most; a power of two
 constexpr int kMaxSpan = 2048;   // places of a CTA, at most
 constexpr int kGradCtas = 148 * 3;  // parts grow while there are as many CTAs
+constexpr int kFinishThreads = 64;
 constexpr int kFillCodes = 8;    // codes of a group in a zero-writing CTA
 constexpr int kLongSpans = 16;   // spans from which a code's partials are added by a whole CTA
 
@@ -620,11 +620,22 @@ __global__ void __launch_bounds__(kGradThreads, kV >= 8 ? 3 : 4) grad_kernel(con
   const int none = (int)a.codes;  // places from the first of this code on are without
   const int64_t p0 = (int64_t)blockIdx.x * a.span;
   const int pitch = a.part + kPad;
-  for (int i = tid; i < a.span; i += kGradThreads) {
+  const int part_shift = 31 - __clz(a.part);
+#pragma unroll 2
+  for (int i = 4 * tid; i < a.span; i += 4 * kGradThreads) {
     const int64_t p = p0 + i;
-    const int at = i + i / a.part * kPad;
-    s_code[at] = p < a.n ? a.sorted[p] : none;
-    s_row[at] = p < a.n ? a.order[p] : 0;
+    int4 c = make_int4(none, none, none, none), r = make_int4(0, 0, 0, 0);
+    if (p + 4 <= a.n) {
+      c = *reinterpret_cast<const int4*>(a.sorted + p);
+      r = *reinterpret_cast<const int4*>(a.order + p);
+    } else {
+      if (p < a.n) c.x = a.sorted[p], r.x = a.order[p];
+      if (p + 1 < a.n) c.y = a.sorted[p + 1], r.y = a.order[p + 1];
+      if (p + 2 < a.n) c.z = a.sorted[p + 2], r.z = a.order[p + 2];
+    }
+    const int at = i + (i >> part_shift) * kPad;
+    *reinterpret_cast<int4*>(s_code + at) = c;
+    *reinterpret_cast<int4*>(s_row + at) = r;
   }
   if (tid < 2) {
     const int64_t p = tid == 0 ? p0 - 1 : p0 + a.span;
@@ -762,14 +773,15 @@ __device__ __forceinline__ void add_partials(const GradArgs& a, int from, int st
 // takes one, and codes over many spans are taken by the whole CTA, group g the
 // spans g, g + groups, ..., then a tree over the groups.
 template <typename TT, int kV>
-__global__ void __launch_bounds__(kGradThreads) grad_finish_kernel(const GradArgs a) {
-  __shared__ int s_long[kGradThreads];
+__global__ void __launch_bounds__(kFinishThreads) grad_finish_kernel(const GradArgs a) {
+  __shared__ int s_long[kFinishThreads];
   __shared__ int s_n_long;
-  __shared__ float s_sum[kV][kGradThreads];
+  __shared__ float s_sum[kV][kFinishThreads];
   sarr::wait_for_previous();
-  const int tid = threadIdx.x, lane = tid & (a.lanes - 1), group = tid / a.lanes;
-  const int groups = kGradThreads / a.lanes;
-  const int v = blockIdx.y * a.lanes + lane;
+  const int lanes = min(a.lanes, kFinishThreads);
+  const int tid = threadIdx.x, lane = tid & (lanes - 1), group = tid / lanes;
+  const int groups = kFinishThreads / lanes;
+  const int v = blockIdx.y * lanes + lane;
   const bool active = v < a.vecs;
   if (tid == 0) s_n_long = 0;
   int first = blockIdx.x * groups + group, last = first, code = (int)a.codes;
@@ -805,7 +817,7 @@ __global__ void __launch_bounds__(kGradThreads) grad_finish_kernel(const GradArg
       __syncthreads();
       if (group < half) {
 #pragma unroll
-        for (int j = 0; j < kV; ++j) s_sum[j][tid] += s_sum[j][tid + half * a.lanes];
+        for (int j = 0; j < kV; ++j) s_sum[j][tid] += s_sum[j][tid + half * lanes];
       }
     }
     __syncthreads();
@@ -1019,9 +1031,12 @@ cudaError_t launch_grad_v(const GradArgs& a, const GradPlan& P, cudaStream_t s) 
   const cudaError_t e = sarr::launch(
       grad_kernel<TG, TT, kV>, {dim3((unsigned)(P.spans + fills), (unsigned)P.tiles), kGradThreads, 0, true, 1}, s, a);
   if (e != cudaSuccess || P.spans <= 1) return e;  // one span: nothing crosses its border
+  const int lanes = std::min(P.lanes, kFinishThreads), at_once = kFinishThreads / lanes;
+  const int64_t borders = P.spans - 1;
   sarr::count_launches(1);
   return sarr::launch(grad_finish_kernel<TT, kV>,
-                      {dim3((unsigned)((P.spans - 1 + groups - 1) / groups), (unsigned)P.tiles), kGradThreads, 0, true, 1},
+                      {dim3((unsigned)((borders + at_once - 1) / at_once), (unsigned)((a.vecs + lanes - 1) / lanes)),
+                       kFinishThreads, 0, true, 1},
                       s, a);
 }
 
@@ -1122,7 +1137,7 @@ extern "C" int sarr_codebook_grad(int64_t n, int64_t codes, int64_t cols, const 
   if (sarr_codebook_grad_workspace_size(n, cols, &need) != SARR_OK) return SARR_ERR_ARG;
   if (codes == 0 || cols == 0) return SARR_OK;
   if (!offsets || (n > 0 && (!order || !sorted_codes))) return SARR_ERR_ARG;
-  if (!aligned(order, 4) || !aligned(sorted_codes, 4) || !aligned(offsets, 4)) return SARR_ERR_ARG;
+  if (!aligned(order, 16) || !aligned(sorted_codes, 16) || !aligned(offsets, 4)) return SARR_ERR_ARG;
   if (!ws || ws_bytes < need || !aligned(ws, 256)) return SARR_ERR_WORKSPACE;
   const int v = vector_of(cols, grad_rows, type_size(rows_type), rows_stride, grad_table, type_size(table_type),
                           table_stride);
