@@ -461,7 +461,7 @@ __global__ void __maxnreg__(kRounds <= 4 ? 32 : 40) sort_scatter_kernel(const So
   if (!a.key_in) sarr::wait_for_previous();
   // where each digit begins, and in it this tile's keys
   {
-    // (the tile's counts are not needed any more: its row of the counts goes there)
+    // (the warps' counts are not needed any more: the tile's row of the counts goes there)
     int32_t* s_before = reinterpret_cast<int32_t*>(S.count);
     const int32_t* before = a.counts + (int64_t)blockIdx.x * bins;
 #pragma unroll 4
@@ -531,13 +531,13 @@ __global__ void __launch_bounds__(256) sort_offsets_kernel(int n, uint32_t codes
 // of its part in order and writes the codes that lie inside it; the sums of
 // codes that cross a part's border are joined through shared memory, those of
 // codes that cross a span's border through the workspace, by grad_finish_kernel.
-// CTAs behind the spans' write the zeros of the codes without Gaussians, while
-// the others wait for their rows.
+// CTAs behind the spans' write the zeros of the codes without Gaussians, while the
+// others wait for their rows (evenly among them they hold the spans up: 39 us
+// against 31 for 16,381 rows of 1024 bf16 into 32,000).
 constexpr int kGradThreads = 256;
 constexpr int kGradRows = 8;     // rows of a group loaded together
-constexpr int kMaxPart = 64;     // places of a group, at most; a power of two
+constexpr int kMaxPart = 64;     // places of a group, at most; a multiple of kGradRows
 constexpr int kMaxSpan = 2048;   // places of a CTA, at most
-constexpr int kGradCtas = 148 * 3;  // parts grow while there are as many CTAs
 constexpr int kFinishThreads = 64;
 constexpr int kFillCodes = 8;    // codes of a group in a zero-writing CTA
 constexpr int kLongSpans = 16;   // spans from which a code's partials are added by a whole CTA
@@ -588,8 +588,9 @@ __global__ void __launch_bounds__(kGradThreads, kV >= 8 ? 3 : 4) grad_kernel(con
   const int groups = kGradThreads / a.lanes;
   const int v = blockIdx.y * a.lanes + lane;
   const bool active = v < a.vecs;
-  if ((int)blockIdx.x >= a.spans) {  // zeros of the codes without Gaussians
-    const int64_t c0 = ((int64_t)blockIdx.x - a.spans) * groups * kFillCodes + group;
+  const int span = blockIdx.x;
+  if (span >= a.spans) {  // zeros of the codes without Gaussians
+    const int64_t c0 = ((int64_t)span - a.spans) * groups * kFillCodes + group;
     bool none[kFillCodes];
 #pragma unroll
     for (int k = 0; k < kFillCodes; ++k) {
@@ -618,12 +619,11 @@ __global__ void __launch_bounds__(kGradThreads, kV >= 8 ? 3 : 4) grad_kernel(con
     return;
   }
   const int none = (int)a.codes;  // places from the first of this code on are without
-  const int64_t p0 = (int64_t)blockIdx.x * a.span;
+  const int64_t p0 = (int64_t)span * a.span;
   const int pitch = a.part + kPad;
-  const int part_shift = 31 - __clz(a.part);
 #pragma unroll 2
-  for (int i = 4 * tid; i < a.span; i += 4 * kGradThreads) {
-    const int64_t p = p0 + i;
+  for (int i = 4 * lane; i < a.part; i += 4 * a.lanes) {
+    const int64_t p = p0 + group * a.part + i;
     int4 c = make_int4(none, none, none, none), r = make_int4(0, 0, 0, 0);
     if (p + 4 <= a.n) {
       c = *reinterpret_cast<const int4*>(a.sorted + p);
@@ -633,9 +633,8 @@ __global__ void __launch_bounds__(kGradThreads, kV >= 8 ? 3 : 4) grad_kernel(con
       if (p + 1 < a.n) c.y = a.sorted[p + 1], r.y = a.order[p + 1];
       if (p + 2 < a.n) c.z = a.sorted[p + 2], r.z = a.order[p + 2];
     }
-    const int at = i + (i >> part_shift) * kPad;
-    *reinterpret_cast<int4*>(s_code + at) = c;
-    *reinterpret_cast<int4*>(s_row + at) = r;
+    *reinterpret_cast<int4*>(s_code + group * pitch + i) = c;
+    *reinterpret_cast<int4*>(s_row + group * pitch + i) = r;
   }
   if (tid < 2) {
     const int64_t p = tid == 0 ? p0 - 1 : p0 + a.span;
@@ -723,7 +722,7 @@ __global__ void __launch_bounds__(kGradThreads, kV >= 8 ? 3 : 4) grad_kernel(con
     float x[kV];
 #pragma unroll
     for (int j = 0; j < kV; ++j) x[j] = s_head[j][tid];
-    store_vec<float, kV>(partial_at<kV>(a, blockIdx.x, 0, v), x);
+    store_vec<float, kV>(partial_at<kV>(a, span, 0, v), x);
   }
   // the group where an open code begins (or the span's first) adds its pieces
   if ((state & kTail) || (group == 0 && (state & kThrough))) {
@@ -741,17 +740,16 @@ __global__ void __launch_bounds__(kGradThreads, kV >= 8 ? 3 : 4) grad_kernel(con
     if (closed && !(state & kThrough)) {
       write_row<TT, kV>(a, (uint32_t)cur, v, acc);
     } else {
-      store_vec<float, kV>(partial_at<kV>(a, blockIdx.x, closed ? 0 : 1, v), acc);
+      store_vec<float, kV>(partial_at<kV>(a, span, closed ? 0 : 1, v), acc);
     }
   }
 }
 
 // Adds the partials of the spans from, from + step, ... of a code whose last span
 // is `last` (where it is the one open at the start).
-template <int kV>
+template <int kAtOnce, int kV>
 __device__ __forceinline__ void add_partials(const GradArgs& a, int from, int step, int last, int v,
                                              float (&acc)[kV]) {
-  constexpr int kAtOnce = 4;
   for (int s0 = from; s0 <= last; s0 += kAtOnce * step) {
     Raw<float, kV> x[kAtOnce];
 #pragma unroll
@@ -800,7 +798,7 @@ __global__ void __launch_bounds__(kFinishThreads) grad_finish_kernel(const GradA
 #pragma unroll
   for (int j = 0; j < kV; ++j) acc[j] = 0.0f;
   if (last > first && !is_long && active) {
-    add_partials<kV>(a, first, 1, last, v, acc);
+    add_partials<4, kV>(a, first, 1, last, v, acc);
     write_row<TT, kV>(a, (uint32_t)code, v, acc);
   }
   const int n_long = s_n_long;
@@ -810,7 +808,7 @@ __global__ void __launch_bounds__(kFinishThreads) grad_finish_kernel(const GradA
     last = (a.offsets[code + 1] - 1) / a.span;
 #pragma unroll
     for (int j = 0; j < kV; ++j) acc[j] = 0.0f;
-    if (active) add_partials<kV>(a, first + group, groups, last, v, acc);
+    if (active) add_partials<8, kV>(a, first + group, groups, last, v, acc);
 #pragma unroll
     for (int j = 0; j < kV; ++j) s_sum[j][tid] = acc[j];
     for (int half = groups / 2; half > 0; half /= 2) {
@@ -993,18 +991,19 @@ struct GradPlan {
 };
 
 // Widths of a group and a part from the sizes alone (the workspace's size is
-// asked for without the arrays): 4 rows wide at least, and parts short enough
-// to fill the GPU with CTAs.
-GradPlan grad_plan(int64_t n, int64_t cols, int64_t vecs) {
+// asked for without the arrays): parts as short as the CTAs that the GPU holds
+// at once can share, so that all spans run side by side, up to kMaxPart.
+constexpr int grad_ctas(int v) { return 148 * (v >= 8 ? 3 : 4); }  // of grad_kernel's launch bounds
+
+GradPlan grad_plan(int64_t n, int64_t cols, int v) {
   GradPlan P;
+  const int64_t vecs = std::max<int64_t>(cols / v, 1);
   P.lanes = pow2_at_least(vecs, kGradThreads);
   P.tiles = (vecs + P.lanes - 1) / P.lanes;
-  const int groups = kGradThreads / P.lanes;
-  P.part = kGradRows;
-  while (P.part < kMaxPart && P.part * 2 * groups <= kMaxSpan &&
-         n / ((int64_t)P.part * 2 * groups) * P.tiles >= kGradCtas)
-    P.part *= 2;
-  P.span = P.part * groups;
+  const int64_t groups = kGradThreads / P.lanes, spans = std::max<int64_t>(grad_ctas(v) / P.tiles, 1);
+  const int64_t share = (n + groups * spans - 1) / (groups * spans), most = std::min<int64_t>(kMaxPart, kMaxSpan / groups);
+  P.part = (int)std::max<int64_t>(std::min((share + kGradRows - 1) / kGradRows * kGradRows, most), kGradRows);
+  P.span = P.part * (int)groups;
   P.spans = (n + P.span - 1) / P.span;
   P.bytes = round256((size_t)P.spans * 2 * (size_t)cols * 4) + 256;
   return P;
@@ -1122,7 +1121,7 @@ extern "C" int sarr_codebook_grad_workspace_size(int64_t n, int64_t cols, size_t
   // the shortest spans that any vector width of these columns gives
   size_t most = 256;
   for (const int v : {1, 2, 4, 8})
-    if (cols % v == 0) most = std::max(most, grad_plan(n, cols, std::max<int64_t>(cols / v, 1)).bytes);
+    if (cols % v == 0) most = std::max(most, grad_plan(n, cols, v).bytes);
   *bytes = most;
   return SARR_OK;
 }
@@ -1141,7 +1140,7 @@ extern "C" int sarr_codebook_grad(int64_t n, int64_t codes, int64_t cols, const 
   if (!ws || ws_bytes < need || !aligned(ws, 256)) return SARR_ERR_WORKSPACE;
   const int v = vector_of(cols, grad_rows, type_size(rows_type), rows_stride, grad_table, type_size(table_type),
                           table_stride);
-  const GradPlan P = grad_plan(n, cols, cols / v);
+  const GradPlan P = grad_plan(n, cols, v);
   GradArgs a;
   memset(&a, 0, sizeof(a));
   a.n = (int)n;
