@@ -169,23 +169,25 @@ def adam_step_clipped(param, grad, exp_avg, exp_avg_sq, segments, step, max_norm
     the gradient clipped by its 2-norm (the gradient itself is not rewritten);
     `segments` = [(end, lr), ...] with ascending ends that cover the buffers, as
     in _native.adam_step; `step` counts from 1. Returns the norm."""
-    names = ("param", "grad", "exp_avg", "exp_avg_sq")
-    tensors = [_native._as_cuda_f32(x, nm) for x, nm in zip((param, grad, exp_avg, exp_avg_sq), names)]
-    count, dev = tensors[0].numel(), tensors[0].device
-    for t, nm in zip(tensors, names):
-        if t.numel() != count or not t.is_contiguous() or t.device != dev:
+    tensors = (param, grad, exp_avg, exp_avg_sq)
+    for t, name in zip(tensors, ("param", "grad", "exp_avg", "exp_avg_sq")):
+        _native._as_cuda_f32(t, name)
+        if t.numel() != param.numel() or not t.is_contiguous() or t.device != param.device:
             raise RuntimeError("Adam buffers must be contiguous, of equal length and on one device")
-    ends = [int(e) for e, _ in segments]
-    begins = [0] + ends[:-1]
-    if not ends or len(ends) > MAX_RANGES or ends[-1] != count or any(b > e for b, e in zip(begins, ends)):
+    count, dev = param.numel(), param.device
+    ranges, at = [], 0
+    for end, lr in segments:
+        ranges.append((at, int(end), at, lr))
+        if end < at:
+            break
+        at = int(end)
+    if not ranges or len(ranges) > MAX_RANGES or at != count or ranges[-1][1] != count:
         raise RuntimeError(f"segments must be 1 to {MAX_RANGES} ascending ends, the last one the buffers' {count}")
-    if not float(max_norm) >= 0.0:
+    if not max_norm >= 0.0:
         raise RuntimeError(f"max_norm must be >= 0, got {max_norm}")
     with _native._on(dev):
-        ws = _workspace(MAX_RANGES, dev)
         norm = torch.empty((), dtype=torch.float32, device=dev)
-        adam_ranges_clipped(tensors, list(zip(begins, ends, begins, [lr for _, lr in segments])), step, max_norm,
-                            betas, eps, norm, ws)
+        adam_ranges_clipped(tensors, ranges, step, max_norm, betas, eps, norm, _workspace(MAX_RANGES, dev))
     return norm
 
 
@@ -193,10 +195,8 @@ def adam_ranges_clipped(tensors, ranges, step, max_norm, betas, eps, norm, ws):
     """sarr_adam_step_clipped on the current device: `tensors` = param, grad,
     exp_avg, exp_avg_sq (flat float32), `ranges` = [(begin, end, first gradient,
     lr), ...], `norm` a float32 scalar to write, `ws` the workspace."""
-    begin = array("q", [r[0] for r in ranges])
-    end = array("q", [r[1] for r in ranges])
-    first = array("q", [r[2] for r in ranges])
-    lr = array("d", [float(r[3]) for r in ranges])
+    begin, end, first, lr = zip(*ranges)
+    begin, end, first, lr = array("q", begin), array("q", end), array("q", first), array("d", lr)
     _native._check(_native.lib().sarr_adam_step_clipped(
         len(ranges), _at(begin), _at(end), _at(first), _at(lr), *[t.data_ptr() for t in tensors],
         float(betas[0]), float(betas[1]), float(eps), int(step), float(max_norm), norm.data_ptr(),
