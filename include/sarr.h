@@ -215,7 +215,7 @@ int sarr_adam_step_ranges(int n_ranges, const int64_t *range_begin, const int64_
  *   index  [n], index_bits 32 or 64; table [codes, cols] in table_type, rows
  *          [n, cols] in rows_type (table_type or SARR_F32), both with a row
  *          stride in elements >= cols; the product is formed in 32 bits and
- *          rounded once. rows must not overlap table. cols <= 2^22.
+ *          rounded once. rows must not overlap table. cols <= 2^21.
  */
 int sarr_codebook_lookup(int64_t n, int64_t codes, int64_t cols, const void *index, int index_bits,
                          const void *table, int table_type, int64_t table_stride, float scale,

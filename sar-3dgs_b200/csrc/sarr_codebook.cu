@@ -640,17 +640,25 @@ __global__ void __launch_bounds__(kGradThreads, kV >= 8 ? 3 : 4) grad_kernel(con
 #pragma unroll 2
   for (int i = 4 * lane; i < a.part; i += 4 * a.lanes) {
     const int64_t p = p0 + group * a.part + i;
-    int4 c = make_int4(none, none, none, none), r = make_int4(0, 0, 0, 0);
+    int c[4], r[4];
     if (p + 4 <= a.n) {
-      c = *reinterpret_cast<const int4*>(a.sorted + p);
-      r = *reinterpret_cast<const int4*>(a.order + p);
+      const int4 c4 = *reinterpret_cast<const int4*>(a.sorted + p), r4 = *reinterpret_cast<const int4*>(a.order + p);
+      c[0] = c4.x, c[1] = c4.y, c[2] = c4.z, c[3] = c4.w;
+      r[0] = r4.x, r[1] = r4.y, r[2] = r4.z, r[3] = r4.w;
     } else {
-      if (p < a.n) c.x = a.sorted[p], r.x = a.order[p];
-      if (p + 1 < a.n) c.y = a.sorted[p + 1], r.y = a.order[p + 1];
-      if (p + 2 < a.n) c.z = a.sorted[p + 2], r.z = a.order[p + 2];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        c[k] = p + k < a.n ? a.sorted[p + k] : none;
+        r[k] = p + k < a.n ? a.order[p + k] : 0;
+      }
     }
-    *reinterpret_cast<int4*>(s_code + group * pitch + i) = c;
-    *reinterpret_cast<int4*>(s_row + group * pitch + i) = r;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {  // whatever the caller's arrays hold, inside the table and the rows
+      c[k] = min((uint32_t)c[k], a.codes);
+      r[k] = min((uint32_t)r[k], (uint32_t)a.n - 1);
+    }
+    *reinterpret_cast<int4*>(s_code + group * pitch + i) = make_int4(c[0], c[1], c[2], c[3]);
+    *reinterpret_cast<int4*>(s_row + group * pitch + i) = make_int4(r[0], r[1], r[2], r[3]);
   }
   if (tid < 2) {
     const int64_t p = tid == 0 ? p0 - 1 : p0 + a.span;
@@ -782,6 +790,10 @@ __device__ __forceinline__ void add_partials(const GradArgs& a, int from, int st
   }
 }
 
+__device__ __forceinline__ int last_span(const GradArgs& a, int code) {
+  return min((a.offsets[code + 1] - 1) / a.span, a.spans - 1);
+}
+
 // Codes over several spans: the sum of their partials, in the order of the
 // spans. Each is found at the border behind the span where it begins; a group
 // takes one, and codes over many spans are taken by the whole CTA, group g the
@@ -802,8 +814,8 @@ __global__ void __launch_bounds__(kFinishThreads) grad_finish_kernel(const GradA
   if (first < a.spans - 1) {
     const int64_t border = (int64_t)(first + 1) * a.span;
     code = a.sorted[border - 1];
-    if (code < (int)a.codes && a.sorted[border] == code && a.offsets[code] / a.span == first)
-      last = (a.offsets[code + 1] - 1) / a.span;
+    if ((uint32_t)code < a.codes && a.sorted[border] == code && a.offsets[code] / a.span == first)
+      last = last_span(a, code);
   }
   const bool is_long = last - first >= kLongSpans;
   if (__syncthreads_or(is_long)) {
@@ -821,7 +833,7 @@ __global__ void __launch_bounds__(kFinishThreads) grad_finish_kernel(const GradA
   for (int k = 0; k < n_long; ++k) {  // the order of these codes does not matter
     code = s_long[k];
     first = a.offsets[code] / a.span;
-    last = (a.offsets[code + 1] - 1) / a.span;
+    last = last_span(a, code);
 #pragma unroll
     for (int j = 0; j < kV; ++j) acc[j] = 0.0f;
     if (active) add_partials<8, kV>(a, first + group, groups, last, v, acc);
@@ -853,7 +865,7 @@ int cuda_status(cudaError_t e) {
   return e == cudaSuccess ? SARR_OK : SARR_ERR_CUDA;
 }
 
-constexpr int64_t kMaxCols = 1 << 22;
+constexpr int64_t kMaxCols = 1 << 21;
 constexpr int64_t kMaxCount = 2147483647 - (1 << 19);  // Gaussians and codes
 
 size_t round256(size_t b) { return (b + 255) & ~(size_t)255; }

@@ -175,8 +175,10 @@ def gradient(grad_rows: torch.Tensor, index: torch.Tensor, codes: int, scale: fl
     """The table's gradient [codes, cols] of lookup(table, index, scale) from the
     rows' gradients [*index.shape, cols] (sort_by_code and gradient_sorted in one
     call)."""
-    if isinstance(grad_rows, torch.Tensor) and grad_rows.dim() > 2:
-        grad_rows = grad_rows.reshape(-1, grad_rows.shape[-1])
+    if isinstance(grad_rows, torch.Tensor) and isinstance(index, torch.Tensor) and grad_rows.dim() not in (0, 2):
+        if grad_rows.shape[:-1] != index.shape:
+            raise RuntimeError(f"grad_rows is {tuple(grad_rows.shape)}, index {tuple(index.shape)}")
+        grad_rows = grad_rows.reshape(index.numel(), grad_rows.shape[-1])
     rows, rows_stride = _matrix(grad_rows, "grad_rows")
     index = _index(index)
     dev, codes = rows.device, int(codes)

@@ -141,8 +141,8 @@ class ViewParallelTrainer:
     sh_index [n]: the SH rows come from a codebook that the Gaussians share
     (cuda_rasterizer.codebook). `sh` is then the table [codes, K], which is
     what is trained (the flat buffer is means | logits | table), and Gaussian
-    i renders sh_scale * sh[sh_index[i]] (zeros for index -1). The index is
-    fixed for the trainer's life, so it is sorted once; each step looks the
+    i renders sh_scale * sh[sh_index[i]] (zeros for index -1). The index (the
+    same on every rank) is fixed for the trainer's life, so it is sorted once; each step looks the
     rows up, and sums their gradients over the codes after the last bucket's
     rows (one all-reduce more, of the table).
 

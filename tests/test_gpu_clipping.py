@@ -291,3 +291,37 @@ def test_more_than_32_bits_of_elements():
     big[3], big[-1] = 3.0, 4.0
     assert float(clipping.clip_grads([big], 1.0)) == 5.0
     assert abs(float(big[-1]) - 0.8) <= 0.8 * 2 ** -11 + 1e-6 and abs(float(big[3]) - 0.6) <= 0.6 * 2 ** -11 + 1e-6
+
+
+def test_in_place_by_name_and_mixed_destinations():
+    """out = the list itself is in place; a list may mix tensors clipped in place and into others."""
+    grads = _list([1000, 2003, 70], (F32, BF16), 20)
+    keep = [g.clone() for g in grads]
+    coef = _coef(_norm64(keep), 0.5)
+    clipping.clip_grads(grads, 0.5, out=grads)
+    _check_clipped(grads, keep, coef)
+    grads = [k.clone() for k in keep]
+    outs = [grads[0], torch.empty(2003, device="cuda"), grads[2]]
+    clipping.clip_grads(grads, 0.5, out=outs)
+    _check_clipped(outs, keep, coef)
+    assert torch.equal(grads[1], keep[1])
+
+
+def test_current_stream_of_the_call():
+    side = torch.cuda.Stream()
+    grads = _list([300000, 7], (F32,), 21)
+    want = clipping.grad_norm(grads)
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for _ in range(4):
+            clipping.grad_norm([torch.zeros(1000000, device="cuda")])
+        with torch.cuda.stream(side):
+            mine = [g.clone() for g in grads]
+            norm = clipping.clip_grads(mine, 1.0)
+            after = clipping.grad_norm(mine)
+            assert torch.equal(norm, want) and abs(float(after) - 1.0) <= 1e-5
+
+
+def test_clipped_adam_of_nothing():
+    e = [torch.zeros(0, device="cuda") for _ in range(4)]
+    assert float(clipping.adam_step_clipped(*e, [(0, 1e-3)], 1, 1.0)) == 0.0

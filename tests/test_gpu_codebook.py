@@ -292,3 +292,73 @@ def test_streams_and_graphs():
             assert torch.equal(outs[k][0], want[k][0]) and torch.equal(outs[k][1], want[k][1])
     for e in eager:
         assert torch.equal(e[0], want[2][0]) and torch.equal(e[1], want[2][1])
+
+
+@pytest.mark.parametrize("shape", [(), (0,), (0, 3), (1,), (2, 0, 4), (2, 3)])
+def test_autograd_of_every_index_shape(shape):
+    """No axis, no element, several axes; an expanded incoming gradient (of a plain sum)."""
+    table = torch.randn(6, 5, generator=_gen(40), device="cuda", requires_grad=True)
+    index = torch.randint(-1, 6, shape, generator=_gen(41), device="cuda")
+    rows = codebook.lookup(table, index, 0.5)
+    assert rows.shape == (*shape, 5)
+    rows.sum().backward()
+    ok, i = _valid(index, 6)
+    want = 0.5 * torch.bincount(i[ok], minlength=6).double()[:, None].expand(6, 5)
+    assert torch.equal(table.grad.double(), want)
+    with pytest.raises(RuntimeError):
+        codebook.gradient(torch.zeros(7, 3, 5, device="cuda"), torch.zeros(7, dtype=torch.int64, device="cuda"), 6)
+
+
+def test_captured_backward():
+    """A whole forward and backward in a graph, replayed on new values."""
+    table = torch.randn(300, 16, generator=_gen(42), device="cuda", requires_grad=True)
+    index = torch.randint(0, 300, (5000,), generator=_gen(43), device="cuda")
+    weight = torch.randn(5000, 16, generator=_gen(44), device="cuda")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            torch.autograd.grad((codebook.lookup(table, index, 2.0) * weight).sum(), table)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        (got,) = torch.autograd.grad((codebook.lookup(table, index, 2.0) * weight).sum(), table)
+    for seed in (45, 46):
+        weight.copy_(torch.randn(5000, 16, generator=_gen(seed), device="cuda"))
+        graph.replay()
+        assert torch.equal(got, codebook.gradient(weight, index, 300, 2.0))
+
+
+def test_order_of_another_index_stays_inside():
+    """An order that was not made for these rows gives wrong sums, and touches nothing outside the table and the rows."""
+    n, codes = 5000, 50
+    order = codebook.sort_by_code(_index(n, codes, 50), codes)
+    rows = torch.randn(n, 16, generator=_gen(51), device="cuda")
+    g = _gen(52)
+    wild = [torch.randint(-2 ** 31, 2 ** 31 - 1, (t.numel(),), generator=g, device="cuda").int() for t in order]
+    around = torch.full((codes + 2, 16), 3.0, device="cuda")
+    for bad in (codebook.SortedCodes(wild[0], order.codes, order.offsets), codebook.SortedCodes(order.order, wild[1], order.offsets)):
+        codebook.gradient_sorted(rows, bad, out=around[1:-1])
+        torch.cuda.synchronize()
+        assert (around[0] == 3).all() and (around[-1] == 3).all()
+    # places that are not aligned to 16 bytes are refused
+    shifted = torch.empty(n + 1, dtype=torch.int32, device="cuda")[1:].copy_(order.order)
+    with pytest.raises(RuntimeError):
+        codebook.gradient_sorted(rows, codebook.SortedCodes(shifted, order.codes, order.offsets))
+
+
+def test_current_stream_of_the_call():
+    """Inputs made and outputs read on a side stream, while the default stream is busy with other calls."""
+    n, codes = 60000, 700
+    index, table = _index(n, codes, 60), torch.randn(codes, 16, generator=_gen(61), device="cuda")
+    rows = torch.randn(n, 16, generator=_gen(62), device="cuda")
+    want = codebook.lookup(table, index, 2.0), codebook.gradient(rows, index, codes)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    for _ in range(5):
+        for _ in range(4):
+            codebook.gradient(rows, index.flip(0).contiguous(), codes)
+        with torch.cuda.stream(side):
+            i, t, r = index.clone(), table.clone(), rows.clone()
+            got = codebook.lookup(t, i, 2.0), codebook.gradient(r, i, codes)
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
