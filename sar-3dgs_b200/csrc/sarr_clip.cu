@@ -492,7 +492,7 @@ cudaError_t norm_group(const ListArgs& a, int begin, int end, bool dependent, do
   fill_list(L, a, begin, end, kNormThreads * kNormVecs * 16);
   if (L.n == 0) return cudaSuccess;
   const unsigned ctas = (unsigned)ctas_for(L.pieces);
-  const cudaError_t e = sarr::launch(norm_kernel<kMax, kInf>, {dim3(ctas), kNormThreads, 0, dependent, 1}, s, L,
+  const cudaError_t e = sarr::launch(norm_kernel<kMax, kInf>, {dim3(ctas), kNormThreads, 0, dependent}, s, L,
                                      partial + *n_partial);
   *n_partial += (int)ctas;
   sarr::count_launches(1);
@@ -507,7 +507,7 @@ cudaError_t clip_group(const ListArgs& a, int begin, int end, const double* part
   if (L.n == 0) return cudaSuccess;
   const unsigned ctas = (unsigned)std::min<int64_t>(L.pieces, kClipCtas);
   sarr::count_launches(1);
-  return sarr::launch(clip_kernel<kMax, kInf>, {dim3(ctas), kThreads, 0, true, 1}, s, L, partial, n_partial,
+  return sarr::launch(clip_kernel<kMax, kInf>, {dim3(ctas), kThreads, 0, true}, s, L, partial, n_partial,
                       max_norm, norm_out);
 }
 
@@ -529,7 +529,7 @@ cudaError_t run_list(const ListArgs& a, double max_norm, float* norm_out, double
   if (!a.outs || n_partial == 0) {
     if (!norm_out) return cudaSuccess;
     sarr::count_launches(1);
-    return sarr::launch(finish_kernel<kInf>, {dim3(1), kThreads, 0, dependent, 1}, s, partial, n_partial, norm_out);
+    return sarr::launch(finish_kernel<kInf>, {dim3(1), kThreads, 0, dependent}, s, partial, n_partial, norm_out);
   }
   float* out = norm_out;
   for (int b = 0; b < a.n; b += kLargeList) {
@@ -647,6 +647,6 @@ extern "C" int sarr_adam_step_clipped(int n_ranges, const int64_t* range_begin, 
   if (e != cudaSuccess) return cuda_status(e);
   const unsigned ctas = (unsigned)std::min<int64_t>(A.pieces, kAdamCtas);
   sarr::count_launches(1);
-  return cuda_status(sarr::launch(adam_kernel, {dim3(ctas), kThreads, 0, true, 1}, s, A, partial, n_partial,
+  return cuda_status(sarr::launch(adam_kernel, {dim3(ctas), kThreads, 0, true}, s, A, partial, n_partial,
                                   max_norm, param, grad, exp_avg, exp_avg_sq, norm_out));
 }

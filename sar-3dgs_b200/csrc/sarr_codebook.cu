@@ -895,7 +895,7 @@ int vector_of(int64_t cols, const void* a, int a_size, int64_t a_stride, const v
 template <typename TI, typename TT, typename TR>
 cudaError_t launch_lookup(const LookupArgs& a, int v, cudaStream_t s) {
   const int64_t per_cta = (int64_t)(kLookupThreads / a.lanes) * kLookupRows;
-  const sarr::LaunchShape shape{dim3((unsigned)((a.n + per_cta - 1) / per_cta)), kLookupThreads, 0, false, 1};
+  const sarr::LaunchShape shape{dim3((unsigned)((a.n + per_cta - 1) / per_cta)), kLookupThreads, 0, false};
   sarr::count_launches(1);
   if (v == 16 / (int)sizeof(TR)) return sarr::launch(lookup_kernel<TI, TT, TR, 16 / (int)sizeof(TR)>, shape, s, a);
   if (v == 2) return sarr::launch(lookup_kernel<TI, TT, TR, 2>, shape, s, a);
@@ -942,9 +942,11 @@ SortPlan sort_plan(int64_t n, int64_t codes) {
 // device, asked for once.
 template <int kRounds>
 cudaError_t allow_tile_smem() {
-  const cudaError_t e = cudaFuncSetAttribute(sort_tile_kernel<kRounds>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             (int)sizeof(TileShared<kRounds>));
-  if (e != cudaSuccess) return e;
+  if constexpr (kRounds <= kOneTile) {
+    const cudaError_t e = cudaFuncSetAttribute(sort_tile_kernel<kRounds>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               (int)sizeof(TileShared<kRounds>));
+    if (e != cudaSuccess) return e;
+  }
   return cudaFuncSetAttribute(sort_scatter_kernel<kRounds>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                               (int)(sizeof(TileShared<kRounds>) + 4 * kMaxBins));
 }
@@ -965,7 +967,7 @@ cudaError_t allow_sort_smem() {
 
 cudaError_t launch_offsets(const SortArgs& a, const int32_t* sorted, int32_t* offsets, cudaStream_t s) {
   sarr::count_launches(1);
-  return sarr::launch(sort_offsets_kernel, {dim3((unsigned)(((int64_t)a.codes + 256) / 256)), 256, 0, true, 1}, s, a.n,
+  return sarr::launch(sort_offsets_kernel, {dim3((unsigned)(((int64_t)a.codes + 256) / 256)), 256, 0, true}, s, a.n,
                       a.codes, sorted, offsets);
 }
 
@@ -974,14 +976,16 @@ cudaError_t run_sort(SortArgs a, const SortPlan& P, char* w, int32_t* order, int
                      cudaStream_t s) {
   constexpr size_t kSmem = sizeof(TileShared<kRounds>);
   a.whole = P.bits <= kWholeBits;
-  if (P.one) {
-    a.key_out = reinterpret_cast<uint32_t*>(sorted);
-    a.place_out = order;
-    a.offsets = P.passes == 1 ? offsets : nullptr;  // more codes than one CTA finds quickly: below
-    a.bits = P.bits;
-    sarr::count_launches(1);
-    const cudaError_t e = sarr::launch(sort_tile_kernel<kRounds>, {dim3(1), kSortThreads, kSmem, false, 1}, s, a);
-    return e != cudaSuccess || P.passes == 1 ? e : launch_offsets(a, sorted, offsets, s);
+  if constexpr (kRounds <= kOneTile) {
+    if (P.one) {
+      a.key_out = reinterpret_cast<uint32_t*>(sorted);
+      a.place_out = order;
+      a.offsets = P.passes == 1 ? offsets : nullptr;  // more codes than one CTA finds quickly: below
+      a.bits = P.bits;
+      sarr::count_launches(1);
+      const cudaError_t e = sarr::launch(sort_tile_kernel<kRounds>, {dim3(1), kSortThreads, kSmem, false}, s, a);
+      return e != cudaSuccess || P.passes == 1 ? e : launch_offsets(a, sorted, offsets, s);
+    }
   }
   a.tiles = P.tiles;
   a.counts = reinterpret_cast<int32_t*>(w + P.counts_at);
@@ -999,16 +1003,16 @@ cudaError_t run_sort(SortArgs a, const SortPlan& P, char* w, int32_t* order, int
     a.bins = P.passes == 1 ? (int)a.codes + 1 : 1 << a.bits;
     const unsigned bins = (unsigned)a.bins, tiles = (unsigned)P.tiles;
     sarr::count_launches(2);
-    e = sarr::launch(sort_histogram_kernel<kRounds>, {dim3(tiles), (unsigned)kCountThreads<kRounds>, 0, p > 0, 1}, s, a);
+    e = sarr::launch(sort_histogram_kernel<kRounds>, {dim3(tiles), (unsigned)kCountThreads<kRounds>, 0, p > 0}, s, a);
     if (e != cudaSuccess) return e;
     a.totals = nullptr;
     if ((int64_t)tiles * bins > kDirectCounts) {
       a.totals = reinterpret_cast<int32_t*>(w + P.totals_at);
       sarr::count_launches(1);
-      e = sarr::launch(sort_prefix_kernel, {dim3((bins + kPrefixBins - 1) / kPrefixBins), kPrefixThreads, 0, true, 1}, s, a);
+      e = sarr::launch(sort_prefix_kernel, {dim3((bins + kPrefixBins - 1) / kPrefixBins), kPrefixThreads, 0, true}, s, a);
       if (e != cudaSuccess) return e;
     }
-    e = sarr::launch(sort_scatter_kernel<kRounds>, {dim3(tiles), kSortThreads, kSmem + 4 * bins, true, 1}, s, a);
+    e = sarr::launch(sort_scatter_kernel<kRounds>, {dim3(tiles), kSortThreads, kSmem + 4 * bins, true}, s, a);
     if (e != cudaSuccess) return e;
     a.key_in = key;
     a.place_in = place;
@@ -1063,14 +1067,14 @@ cudaError_t launch_grad_v(const GradArgs& a, const GradPlan& P, cudaStream_t s) 
   const int64_t fills = ((int64_t)a.codes + groups * kFillCodes - 1) / (groups * kFillCodes);
   sarr::count_launches(1);
   const cudaError_t e = sarr::launch(
-      grad_kernel<TG, TT, kV>, {dim3((unsigned)(P.spans + fills), (unsigned)P.tiles), kGradThreads, 0, true, 1}, s, a);
+      grad_kernel<TG, TT, kV>, {dim3((unsigned)(P.spans + fills), (unsigned)P.tiles), kGradThreads, 0, true}, s, a);
   if (e != cudaSuccess || P.spans <= 1) return e;  // one span: nothing crosses its border
   const int lanes = std::min(P.lanes, kFinishThreads), at_once = kFinishThreads / lanes;
   const int64_t borders = P.spans - 1;
   sarr::count_launches(1);
   return sarr::launch(grad_finish_kernel<TT, kV>,
                       {dim3((unsigned)((borders + at_once - 1) / at_once), (unsigned)((a.vecs + lanes - 1) / lanes)),
-                       kFinishThreads, 0, true, 1},
+                       kFinishThreads, 0, true},
                       s, a);
 }
 

@@ -1,6 +1,6 @@
 // Launch helper of the multi-kernel operators (codebook, clipping): a launch
 // that may start before its predecessor on the stream has finished
-// (programmatic dependent launch) and that may group its CTAs into clusters.
+// (programmatic dependent launch).
 #ifndef SARR_LAUNCH_CUH_
 #define SARR_LAUNCH_CUH_
 
@@ -26,14 +26,13 @@ struct LaunchShape {
   dim3 grid;
   unsigned threads;
   size_t smem;
-  bool dependent;    // may start before the previous kernel of the stream ends
-  unsigned cluster;  // CTAs per cluster (1: none)
+  bool dependent;  // may start before the previous kernel of the stream ends
 };
 
 template <typename... KArgs, typename... Args>
 cudaError_t launch(void (*kernel)(KArgs...), const LaunchShape& shape, cudaStream_t stream,
                    Args&&... args) {
-  if (!shape.dependent && shape.cluster <= 1) {  // costs the host less than a launch with attributes
+  if (!shape.dependent) {  // costs the host less than a launch with attributes
     kernel<<<shape.grid, shape.threads, shape.smem, stream>>>(static_cast<KArgs>(args)...);
     return cudaGetLastError();
   }
@@ -42,20 +41,11 @@ cudaError_t launch(void (*kernel)(KArgs...), const LaunchShape& shape, cudaStrea
   cfg.blockDim = dim3(shape.threads);
   cfg.dynamicSmemBytes = shape.smem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[2];
-  unsigned n = 0;
-  if (shape.dependent) {
-    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[n++].val.programmaticStreamSerializationAllowed = 1;
-  }
-  if (shape.cluster > 1) {
-    attr[n].id = cudaLaunchAttributeClusterDimension;
-    attr[n].val.clusterDim.x = shape.cluster;
-    attr[n].val.clusterDim.y = 1;
-    attr[n++].val.clusterDim.z = 1;
-  }
-  cfg.attrs = attr;
-  cfg.numAttrs = n;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
 }
 
