@@ -129,6 +129,12 @@ __device__ __forceinline__ uint32_t code_of(const void* index, bool wide, int64_
 // ---------------------------------------------------------------------------
 // lookup
 // ---------------------------------------------------------------------------
+// A row is held by `lanes` threads, 16 bytes of the result each, so a warp writes
+// whole lines. Bound by the writes to HBM: 1M rows of 16 floats from 4096 bf16
+// rows take 13.0 us (68 MB, 5.3 TB/s, 0.80 of the measured copy bandwidth), 16,381
+// rows of 1000 bf16 11.9 us (5.5 TB/s). Six rows a thread and CTAs of 64 threads:
+// 12.9 us against 15.6 with 8 and 256 (shorter CTAs fill the tail), 17 with four
+// loads of 32-byte halves; 1000 rows take 2 us, a launch.
 constexpr int kLookupThreads = 64;
 constexpr int kLookupRows = 6;  // rows per thread, their loads in flight together
 
@@ -198,13 +204,20 @@ __global__ void __launch_bounds__(kLookupThreads) lookup_kernel(const LookupArgs
 //              and the earlier tiles (in runs, since the tile is in order). The
 //              first pass sorts its tile before it waits for the other two.
 // With one pass the scan over the totals is the offsets.
+//
+// Bound by integer instructions and latency, not by its 12 bytes a key: 1M keys
+// take 14.6 us for 256 codes (one pass in the tile), 22 for 4096 (two), 42 for
+// 65,536 (two passes over all tiles); 50,000 keys of 1024 codes 9 us, 1000 keys 4 to
+// 7. Votes against a match over the lanes: 22 against 29 us; kernels small enough to
+// share an SM against ones that are not: 22 against 29; 13-bit digits against two
+// passes of 7: 22 against about 30.
 constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32;
 constexpr int kMaxRounds = 8;                          // words per thread
 constexpr int kPlaceBits = 13;                         // of a place in a tile
 constexpr int kLocalBits = 9, kLocalBins = 1 << kLocalBits;  // of a pass inside a tile, at most
 constexpr int kMaxDigitBits = 13, kMaxBins = 1 << kMaxDigitBits;
 constexpr int kWholeBits = 32 - kPlaceBits;            // of a key that fits a word
-constexpr int kOneTile = 4;                            // up to 4096 such keys in one tile
+constexpr int kOneTile = 4;                            // up to 4096 such keys in one tile (8192: 19 us against 10 in 8 tiles)
 constexpr int kPrefixThreads = 256, kPrefixBins = 32;  // bins of a CTA; its threads split the tiles 8 ways
 constexpr int kDirectCounts = 16384;                   // counts that each scatter CTA adds itself, without the prefix kernel
 constexpr int kManyTiles = 148;                        // tiles grow until there are no more of them than SMs
@@ -549,6 +562,12 @@ __global__ void __launch_bounds__(256) sort_offsets_kernel(int n, uint32_t codes
 // CTAs behind the spans' write the zeros of the codes without Gaussians, while the
 // others wait for their rows (evenly among them they hold the spans up: 39 us
 // against 31 for 16,381 rows of 1024 bf16 into 32,000).
+//
+// Bound by the rows' reads. Rows of 1024 bf16: 31 us for 165 MB (5.3 TB/s, 0.81 of
+// the measured copy bandwidth). Rows of 16 floats come as random 64-byte reads: 1M
+// of them 20.6 us (24 where one code has 6 % of them), and the lookup kernel reads
+// 64 MB of random rows in about 20 us too; taken in the order of the sort there is
+// nothing to stream.
 constexpr int kGradThreads = 256;
 constexpr int kGradRows = 8;     // rows of a group loaded together
 constexpr int kMaxPart = 64;     // places of a group, at most; a multiple of kGradRows
