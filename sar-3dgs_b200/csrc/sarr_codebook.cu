@@ -133,8 +133,8 @@ __device__ __forceinline__ uint32_t code_of(const void* index, bool wide, int64_
 // whole lines. Bound by the writes to HBM: 1M rows of 16 floats from 4096 bf16
 // rows take 13.0 us (68 MB, 5.3 TB/s, 0.80 of the measured copy bandwidth), 16,381
 // rows of 1000 bf16 11.9 us (5.5 TB/s). Six rows a thread and CTAs of 64 threads:
-// 12.9 us against 15.6 with 8 and 256 (shorter CTAs fill the tail), 17 with four
-// loads of 32-byte halves; 1000 rows take 2 us, a launch.
+// 12.9 us against 14.1 with 4 and 256 and 15.6 with 8 and 256 (short CTAs fill the
+// tail), 27 where a lane wrote 32 bytes in two halves; 1000 rows take 2 us, a launch.
 constexpr int kLookupThreads = 64;
 constexpr int kLookupRows = 6;  // rows per thread, their loads in flight together
 
@@ -187,8 +187,8 @@ __global__ void __launch_bounds__(kLookupThreads) lookup_kernel(const LookupArgs
 // ---------------------------------------------------------------------------
 // A stable sort of the keys (the codes, `codes` for none). The unit is a tile of
 // 1024 to 8192 keys that one CTA sorts in registers and shared memory, as words
-// digit << 13 | place in the tile: each warp holds a contiguous part of the tile,
-// 32 words a round; a word's rank among the warp's words of its digit is a running
+// key << 13 | place in the tile (the digit alone of a key over 19 bits): each warp
+// holds a contiguous part of the tile, 32 words a round; a word's rank among the warp's words of its digit is a running
 // count plus the lower lanes that vote for the same digit (one vote per bit, so a
 // digit costs the same whatever the keys are), and a scan over the warps' counts
 // and the digits gives every rank its place. Counts are 16 bits wide, two digits
@@ -208,9 +208,8 @@ __global__ void __launch_bounds__(kLookupThreads) lookup_kernel(const LookupArgs
 // Bound by integer instructions and latency, not by its 12 bytes a key: 1M keys
 // take 14.6 us for 256 codes (one pass in the tile), 22 for 4096 (two), 42 for
 // 65,536 (two passes over all tiles); 50,000 keys of 1024 codes 9 us, 1000 keys 4 to
-// 7. Votes against a match over the lanes: 22 against 29 us; kernels small enough to
-// share an SM against ones that are not: 22 against 29; 13-bit digits against two
-// passes of 7: 22 against about 30.
+// 7. For 1M keys of 4096 codes: votes 30 us where a match over the lanes took 36, then
+// 22 with kernels small enough to share an SM where they were not 29.
 constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32;
 constexpr int kMaxRounds = 8;                          // words per thread
 constexpr int kPlaceBits = 13;                         // of a place in a tile
@@ -222,6 +221,7 @@ constexpr int kPrefixThreads = 256, kPrefixBins = 32;  // bins of a CTA; its thr
 constexpr int kDirectCounts = 16384;                   // counts that each scatter CTA adds itself, without the prefix kernel
 constexpr int kManyTiles = 148;                        // tiles grow until there are no more of them than SMs
 static_assert(kSortThreads * kMaxRounds <= 1 << kPlaceBits, "a place fits its bits");
+static_assert(kSortWarps * kLocalBins * sizeof(uint16_t) >= kMaxBins * sizeof(int32_t), "a row of counts fits the warps' counts");
 
 struct SortArgs {
   int n;
