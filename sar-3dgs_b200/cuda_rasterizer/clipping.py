@@ -15,6 +15,7 @@ import ctypes
 import functools
 import math
 from array import array
+from operator import attrgetter
 from typing import Iterable, Optional, Sequence
 
 import torch
@@ -25,6 +26,7 @@ __all__ = ["grad_norm", "clip_grads", "clip_grad_norm_", "adam_step_clipped"]
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _NORMS = {2.0: 0, math.inf: 1}
+_DTYPE = attrgetter("dtype")
 MAX_RANGES = 64  # ranges of one clipped Adam step
 
 
@@ -42,15 +44,18 @@ def _dense(t):
 
 def _list(tensors, name):
     """(pointers, counts, types, device, whether all are contiguous) of dense CUDA tensors."""
-    try:
-        types = [_TYPES[t.dtype] for t in tensors]
-        dev = tensors[0].device
-        contiguous = all([t.is_contiguous() for t in tensors])
-        if (dev.type == "cuda" and [t.get_device() for t in tensors].count(dev.index) == len(tensors)
-                and (contiguous or all([_dense(t) for t in tensors]))):
-            return (array("Q", [t.data_ptr() for t in tensors]), array("q", [t.numel() for t in tensors]),
-                    array("i", types), dev, contiguous)
-    except (AttributeError, KeyError):
+    try:  # unbound methods under map: less host time than a loop, for lists of hundreds
+        n, dtypes, dev = len(tensors), list(map(_DTYPE, tensors)), tensors[0].device
+        contiguous = all(map(torch.Tensor.is_contiguous, tensors))
+        if (dev.type == "cuda" and list(map(torch.Tensor.get_device, tensors)).count(dev.index) == n
+                and (contiguous or all(map(_dense, tensors)))):
+            if dtypes.count(dtypes[0]) == n:
+                types = array("i", [_TYPES[dtypes[0]]]) * n
+            else:
+                types = array("i", map(_TYPES.__getitem__, dtypes))
+            return (array("Q", map(torch.Tensor.data_ptr, tensors)), array("q", map(torch.Tensor.numel, tensors)),
+                    types, dev, contiguous)
+    except (AttributeError, KeyError, TypeError):
         pass
     dev = None
     for k, t in enumerate(tensors):  # find out which
