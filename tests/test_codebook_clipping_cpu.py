@@ -65,8 +65,26 @@ def test_gradient_refusals(kw, status):
     assert _grad(**kw) == status
 
 
+def _gradient(**kw):
+    a = dict(n=4, codes=8, cols=16, rows=D, rtype=0, rstride=16, index=D, bits=64, scale=1.0, table=D, ttype=0, tstride=16,
+             ws=D, ws_bytes=1 << 24)
+    a.update(kw)
+    return _native.lib().sarr_codebook_gradient(*a.values(), None)
+
+
+@pytest.mark.parametrize("kw,status", [
+    (dict(n=-1), ARG), (dict(n=BIG), ARG), (dict(codes=-1), ARG), (dict(cols=2 ** 22), ARG), (dict(bits=16), ARG),
+    (dict(index=None), ARG), (dict(index=ctypes.c_void_p(260)), ARG), (dict(rows=None), ARG), (dict(table=None), ARG),
+    (dict(rtype=2, ttype=1), ARG), (dict(rstride=15), ARG), (dict(tstride=0), ARG), (dict(ws=None), WORKSPACE),
+    (dict(ws_bytes=64), WORKSPACE), (dict(ws=ctypes.c_void_p(384 + 8)), WORKSPACE)])
+def test_gradient_in_one_call_refusals(kw, status):
+    assert _gradient(**kw) == status
+
+
 def test_gradient_of_no_codes():
     assert _grad(codes=0, offsets=None, table=None) == 0
+    assert _gradient(codes=0, table=None) == 0
+    assert _gradient(cols=0, rstride=0, tstride=0) == 0
 
 
 def _clip(grads=(4096, 8192), counts=(16, 16), types=(0, 0), outs=(4096, 8192), otypes=(0, 0), kind=0, max_norm=1.0,
