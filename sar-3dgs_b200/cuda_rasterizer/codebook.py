@@ -6,8 +6,8 @@ Gaussian's 20 trained floats) come from a table that they share, by index.
 `lookup` is differentiable with respect to the table. Its gradient sums the
 rows' gradients of every code in the order of the Gaussians: `gradient` sorts
 the index and sums, `sort_by_code` and `gradient_sorted` are its two halves for
-a caller whose index stays the same over many steps (ViewParallelTrainer with
-`sh_index`). A Gaussian whose index is outside [0, codes) has no code: its row
+a caller whose index stays the same over many steps (`lookup` takes the order
+too; ViewParallelTrainer with `sh_index` keeps one). A Gaussian whose index is outside [0, codes) has no code: its row
 is zeros and its gradient reaches no code.
 
 Tables and rows are float32, bfloat16 or float16 CUDA tensors (rows in the
@@ -200,24 +200,34 @@ def gradient(grad_rows: torch.Tensor, index: torch.Tensor, codes: int, scale: fl
 
 class _Lookup(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, table, index, scale, dtype):
+    def forward(ctx, table, index, scale, dtype, order):
         rows = _lookup(table.detach(), index, scale, dtype)
-        ctx.save_for_backward(index)
+        ctx.save_for_backward(index, *(order or ()))
         ctx.scale, ctx.codes, ctx.dtype = scale, table.shape[0], table.dtype
         return rows
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        (index,) = ctx.saved_tensors
-        return gradient(grad, index, ctx.codes, ctx.scale, ctx.dtype), None, None, None
+        index, *order = ctx.saved_tensors
+        if order:
+            grad = grad.reshape(index.numel(), grad.shape[-1])
+            grad_table = gradient_sorted(grad, SortedCodes(*order), ctx.scale, ctx.dtype)
+        else:
+            grad_table = gradient(grad, index, ctx.codes, ctx.scale, ctx.dtype)
+        return grad_table, None, None, None, None
 
 
 def lookup(table: torch.Tensor, index: torch.Tensor, scale: float = 1.0,
-           dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+           dtype: Optional[torch.dtype] = None, order: Optional[SortedCodes] = None) -> torch.Tensor:
     """rows[i] = scale * table[index[i]] ([*index.shape, cols]; zeros where
     index[i] is outside [0, codes)), in `dtype` (the table's type by default, or
-    float32), with its gradient with respect to the table."""
+    float32), with its gradient with respect to the table. `order`: what
+    sort_by_code gave for this index, where the caller keeps it; without it the
+    gradient sorts the index."""
+    if order is not None and (order.order.numel() != index.numel() or order.offsets.numel() != table.shape[0] + 1):
+        raise RuntimeError(f"order is of {order.order.numel()} Gaussians and {order.offsets.numel() - 1} codes, the "
+                           f"index of {index.numel()} and the table of {table.shape[0]}")
     if isinstance(table, torch.Tensor) and table.requires_grad and torch.is_grad_enabled():
-        return _Lookup.apply(table, index, scale, dtype)
+        return _Lookup.apply(table, index, scale, dtype, order)
     return _lookup(table, index, scale, dtype)

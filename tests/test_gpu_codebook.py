@@ -362,3 +362,18 @@ def test_current_stream_of_the_call():
             i, t, r = index.clone(), table.clone(), rows.clone()
             got = codebook.lookup(t, i, 2.0), codebook.gradient(r, i, codes)
             assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_autograd_with_a_kept_order():
+    index = _index(5000, 60, 70).reshape(50, 100)
+    order = codebook.sort_by_code(index, 60)
+    weight = torch.randn(50, 100, 12, generator=_gen(71), device="cuda")
+    grads = []
+    for o in (None, order):
+        table = torch.randn(60, 12, generator=_gen(72), device="cuda", requires_grad=True)
+        (codebook.lookup(table, index, 0.5, order=o) * weight).sum().backward()
+        grads.append(table.grad)
+    assert torch.equal(grads[0], grads[1]) and float(grads[0].abs().max()) > 0
+    for bad in (codebook.sort_by_code(index[:10], 60), codebook.sort_by_code(index, 61)):
+        with pytest.raises(RuntimeError):
+            codebook.lookup(table, index, order=bad)
