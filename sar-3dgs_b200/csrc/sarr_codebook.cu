@@ -236,7 +236,7 @@ struct SortArgs {
   int shift, bits, bins;     // of this pass's digit; with one pass bins = codes + 1, else 2^bits
   int tiles;
   bool whole;                // words hold the whole key (of up to 19 bits), else the digit
-  int32_t* offsets;          // written by the scatter of a sort of one pass, else null
+  int32_t* starts;           // null, or [bins]: where each digit's keys begin (with one pass: the offsets)
 };
 
 __device__ __forceinline__ uint32_t sort_key(const SortArgs& a, int i) {
@@ -381,7 +381,7 @@ __global__ void __launch_bounds__(kSortThreads) sort_tile_kernel(const SortArgs 
       a.place_out[e] = word[r] & ((1 << kPlaceBits) - 1);
     }
   }
-  if (!a.offsets) return;
+  if (!a.starts) return;
   // the first place whose key is >= c
   for (int64_t c = threadIdx.x; c <= a.codes; c += kSortThreads) {
     int lo = 0, hi = a.n;
@@ -390,7 +390,7 @@ __global__ void __launch_bounds__(kSortThreads) sort_tile_kernel(const SortArgs 
       if (S.word[mid] >> kPlaceBits < (uint32_t)c) lo = mid + 1;
       else hi = mid;
     }
-    a.offsets[c] = lo;
+    a.starts[c] = lo;
   }
 }
 
@@ -508,7 +508,7 @@ __global__ void __maxnreg__(kRounds <= 4 ? 32 : 40) sort_scatter_kernel(const So
     for (int d = first; d < end; ++d) {
       const int x = s_base[d];
       s_base[d] = at + s_before[d];
-      if (a.offsets && blockIdx.x == 0) a.offsets[d] = at;
+      if (a.starts && blockIdx.x == 0) a.starts[d] = at;
       at += x;
     }
   }
@@ -534,14 +534,21 @@ __global__ void __maxnreg__(kRounds <= 4 ? 32 : 40) sort_scatter_kernel(const So
   }
 }
 
-// The first place whose code is >= c, for each c.
+// The first place whose code is >= c, for each c: a search among the keys of its
+// last digit (starts: where each digit's keys begin), or among all.
 __global__ void __launch_bounds__(256) sort_offsets_kernel(int n, uint32_t codes, const int32_t* sorted,
+                                                           const int32_t* starts, int shift, int bins,
                                                            int32_t* offsets) {
   sarr::dependents_may_start();
   sarr::wait_for_previous();
   const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (c > codes) return;
   int lo = 0, hi = n;
+  if (starts) {
+    const int digit = (int)(c >> shift);
+    lo = starts[digit];
+    if (digit + 1 < bins) hi = starts[digit + 1];
+  }
   while (lo < hi) {
     const int mid = lo + (hi - lo) / 2;
     if ((uint32_t)sorted[mid] < (uint32_t)c) lo = mid + 1;
@@ -929,7 +936,7 @@ cudaError_t launch_lookup(const LookupArgs& a, bool wide, int v, cudaStream_t s)
 struct SortPlan {
   int bits, passes, digit_bits, rounds, tiles;
   bool one;  // one tile sorts it
-  size_t key_bytes, counts_at, totals_at, bytes;
+  size_t key_bytes, counts_at, totals_at, starts_at, bytes;
 };
 
 SortPlan sort_plan(int64_t n, int64_t codes) {
@@ -944,7 +951,7 @@ SortPlan sort_plan(int64_t n, int64_t codes) {
   P.rounds = 1;
   while (P.rounds < least && P.rounds < kMaxRounds) P.rounds *= 2;
   P.tiles = (int)((thousands + P.rounds - 1) / P.rounds);
-  P.key_bytes = P.counts_at = P.totals_at = 0;
+  P.key_bytes = P.counts_at = P.totals_at = P.starts_at = 0;
   P.bytes = 0;  // one tile: shared memory holds it all
   P.one = one || n == 0;
   if (!P.one) {
@@ -952,7 +959,8 @@ SortPlan sort_plan(int64_t n, int64_t codes) {
     const int buffers = std::min(P.passes - 1, 2);
     P.counts_at = (size_t)buffers * 2 * P.key_bytes;
     P.totals_at = P.counts_at + round256((size_t)P.tiles * (4u << P.digit_bits));
-    P.bytes = P.totals_at + round256(4u << P.digit_bits);
+    P.starts_at = P.totals_at + round256(4u << P.digit_bits);
+    P.bytes = P.starts_at + round256(4u << P.digit_bits);
   }
   return P;
 }
@@ -987,7 +995,7 @@ cudaError_t allow_sort_smem() {
 cudaError_t launch_offsets(const SortArgs& a, const int32_t* sorted, int32_t* offsets, cudaStream_t s) {
   sarr::count_launches(1);
   return sarr::launch(sort_offsets_kernel, {dim3((unsigned)(((int64_t)a.codes + 256) / 256)), 256, 0, true}, s, a.n,
-                      a.codes, sorted, offsets);
+                      a.codes, sorted, a.starts, a.shift, a.bins, offsets);
 }
 
 template <int kRounds>
@@ -999,7 +1007,7 @@ cudaError_t run_sort(SortArgs a, const SortPlan& P, char* w, int32_t* order, int
     if (P.one) {
       a.key_out = reinterpret_cast<uint32_t*>(sorted);
       a.place_out = order;
-      a.offsets = P.passes == 1 ? offsets : nullptr;  // more codes than one CTA finds quickly: below
+      a.starts = P.passes == 1 ? offsets : nullptr;  // more codes than one CTA finds quickly: below
       a.bits = P.bits;
       sarr::count_launches(1);
       const cudaError_t e = sarr::launch(sort_tile_kernel<kRounds>, {dim3(1), kSortThreads, kSmem, false}, s, a);
@@ -1018,7 +1026,7 @@ cudaError_t run_sort(SortArgs a, const SortPlan& P, char* w, int32_t* order, int
     a.bits = std::min(P.digit_bits, P.bits - a.shift);
     a.key_out = key;
     a.place_out = place;
-    a.offsets = P.passes == 1 ? offsets : nullptr;
+    a.starts = !last ? nullptr : P.passes == 1 ? offsets : reinterpret_cast<int32_t*>(w + P.starts_at);
     a.bins = P.passes == 1 ? (int)a.codes + 1 : 1 << a.bits;
     const unsigned bins = (unsigned)a.bins, tiles = (unsigned)P.tiles;
     sarr::count_launches(2);
