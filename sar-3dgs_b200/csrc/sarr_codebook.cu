@@ -269,18 +269,18 @@ __device__ __forceinline__ int warps_before(const int32_t* warp_sum, int lane, i
 }
 
 // One stable pass over the tile's words, which the threads hold: element
-// (warp * kRounds + r) * 32 + lane in word[r]; elements from len on are none. On
-// return S holds the tile in order and so do the threads.
+// (warp * kRounds + r) * 32 + lane in word[r]. Elements behind the keys are all ones:
+// last in every digit, they stay behind. On return S holds the tile in order and so
+// do the threads.
 template <int kRounds>
-__device__ __forceinline__ void tile_pass(TileShared<kRounds>& S, uint32_t (&word)[kRounds], int len, int shift,
-                                          int bits) {
+__device__ __forceinline__ void tile_pass(TileShared<kRounds>& S, uint32_t (&word)[kRounds], int shift, int bits) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, bins = 1 << bits;
   const int first = warp * kRounds * 32 + lane;
   uint16_t* count = S.count[warp];
   for (int i = lane; i < (bins + 1) / 2; i += 32) reinterpret_cast<uint32_t*>(count)[i] = 0;
   uint32_t peers[kRounds];
 #pragma unroll
-  for (int r = 0; r < kRounds; ++r) peers[r] = __ballot_sync(0xffffffffu, first + 32 * r < len);
+  for (int r = 0; r < kRounds; ++r) peers[r] = 0xffffffffu;
   uint32_t bit = 1u << shift;
   for (int b = 0; b < bits; ++b, bit += bit) {
 #pragma unroll
@@ -291,14 +291,14 @@ __device__ __forceinline__ void tile_pass(TileShared<kRounds>& S, uint32_t (&wor
     }
   }
   __syncwarp();
+  const uint32_t lower = (1u << lane) - 1;
   int rank[kRounds];
 #pragma unroll
   for (int r = 0; r < kRounds; ++r) {
-    const uint32_t digit = (word[r] >> shift) & (bins - 1), below = peers[r] & ((1u << lane) - 1);
-    const bool have = first + 32 * r < len;
-    const int before = have ? count[digit] : 0;
+    const uint32_t digit = (word[r] >> shift) & (bins - 1), below = peers[r] & lower;
+    const int before = count[digit];
     __syncwarp();
-    if (have && below == 0) count[digit] = (uint16_t)(before + __popc(peers[r]));
+    if (below == 0) count[digit] = (uint16_t)(before + __popc(peers[r]));
     __syncwarp();
     rank[r] = before + __popc(below);
   }
@@ -334,15 +334,12 @@ __device__ __forceinline__ void tile_pass(TileShared<kRounds>& S, uint32_t (&wor
   __syncthreads();
 #pragma unroll
   for (int r = 0; r < kRounds; ++r) {
-    if (first + 32 * r < len) {
-      const uint32_t digit = (word[r] >> shift) & (bins - 1);
-      S.word[S.digit[digit] + count[digit] + rank[r]] = word[r];
-    }
+    const uint32_t digit = (word[r] >> shift) & (bins - 1);
+    S.word[S.digit[digit] + count[digit] + rank[r]] = word[r];
   }
   __syncthreads();
 #pragma unroll
-  for (int r = 0; r < kRounds; ++r)
-    if (first + 32 * r < len) word[r] = S.word[first + 32 * r];
+  for (int r = 0; r < kRounds; ++r) word[r] = S.word[first + 32 * r];
 }
 
 // The tile's words into the threads, then sorted by the `bits` bits of the digit.
@@ -356,12 +353,15 @@ __device__ __forceinline__ void sort_tile(const SortArgs& a, TileShared<kRounds>
     word[r] = e < len ? sort_key(a, tile0 + e) : 0;
   }
 #pragma unroll
-  for (int r = 0; r < kRounds; ++r)
-    word[r] = (a.whole ? word[r] : (word[r] >> a.shift) & ((1u << a.bits) - 1)) << kPlaceBits | (first + 32 * r);
+  for (int r = 0; r < kRounds; ++r) {
+    const int e = first + 32 * r;
+    word[r] = (a.whole ? word[r] : (word[r] >> a.shift) & ((1u << a.bits) - 1)) << kPlaceBits | e;
+    if (e >= len) word[r] = 0xffffffffu;
+  }
   const int passes = (a.bits + kLocalBits - 1) / kLocalBits, each = (a.bits + passes - 1) / passes;
 #pragma unroll 1
   for (int p = 0; p < passes; ++p)
-    tile_pass<kRounds>(S, word, len, digit_shift(a) + p * each, min(each, a.bits - p * each));
+    tile_pass<kRounds>(S, word, digit_shift(a) + p * each, min(each, a.bits - p * each));
 }
 
 extern __shared__ __align__(16) unsigned char s_sort[];
