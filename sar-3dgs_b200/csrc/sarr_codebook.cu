@@ -206,7 +206,7 @@ __global__ void __launch_bounds__(kLookupThreads) lookup_kernel(const LookupArgs
 // With one pass the scan over the totals is the offsets.
 //
 // Bound by integer instructions and latency, not by its 12 bytes a key: 1M keys
-// take 14.6 us for 256 codes (one pass in the tile), 22 for 4096 (two), 42 for
+// take 14.4 us for 256 codes (one pass in the tile), 22.5 for 4096 (two), 37 for
 // 65,536 (two passes over all tiles); 50,000 keys of 1024 codes 9 us, 1000 keys 4 to
 // 7. For 1M keys of 4096 codes: votes 30 us where a match over the lanes took 36, then
 // 22 with kernels small enough to share an SM where they were not 29.
@@ -217,7 +217,7 @@ constexpr int kLocalBits = 9, kLocalBins = 1 << kLocalBits;  // of a pass inside
 constexpr int kMaxDigitBits = 13, kMaxBins = 1 << kMaxDigitBits;
 constexpr int kWholeBits = 32 - kPlaceBits;            // of a key that fits a word
 constexpr int kOneTile = 4;                            // up to 4096 such keys in one tile (8192: 19 us against 10 in 8 tiles)
-constexpr int kPrefixThreads = 256, kPrefixBins = 32;  // bins of a CTA; its threads split the tiles 8 ways
+constexpr int kPrefixThreads = 256;                    // of the prefix kernel: 16 bins a CTA, or 32 where that is over a CTA per SM
 constexpr int kDirectCounts = 16384;                   // counts that each scatter CTA adds itself, without the prefix kernel
 constexpr int kManyTiles = 148;                        // tiles grow until there are no more of them than SMs
 static_assert(kSortThreads * kMaxRounds <= 1 << kPlaceBits, "a place fits its bits");
@@ -401,14 +401,13 @@ constexpr int kCountThreads = kRounds >= 8 ? 512 : 256;
 template <int kRounds>
 __global__ void __launch_bounds__(kCountThreads<kRounds>, 2048 / kCountThreads<kRounds>)
     sort_histogram_kernel(const SortArgs a) {
-  constexpr int kTile = kSortThreads * kRounds, kThreads = kCountThreads<kRounds>, kBatch = 4;
+  constexpr int kTile = kSortThreads * kRounds, kThreads = kCountThreads<kRounds>, kBatch = 8;
   __shared__ int32_t s_bin[kMaxBins];
   sarr::dependents_may_start();
   sarr::wait_for_previous();
   const int bins = a.bins, mask = (1 << a.bits) - 1, tile0 = blockIdx.x * kTile, len = min(kTile, a.n - tile0);
   for (int d = threadIdx.x; d < bins; d += kThreads) s_bin[d] = 0;
   __syncthreads();
-#pragma unroll 2
   for (int e0 = threadIdx.x; e0 < len; e0 += kBatch * kThreads) {
     uint32_t key[kBatch];
 #pragma unroll
@@ -422,14 +421,18 @@ __global__ void __launch_bounds__(kCountThreads<kRounds>, 2048 / kCountThreads<k
   for (int d = threadIdx.x; d < bins; d += kThreads) a.counts[(int64_t)blockIdx.x * bins + d] = s_bin[d];
 }
 
-// counts[t][d] becomes the sum of counts[0 .. t-1][d], totals[d] the sum of all.
+// counts[t][d] becomes the sum of counts[0 .. t-1][d], totals[d] the sum of all. A
+// CTA takes kBins digits; its threads split the tiles. Of 1M keys, 65,536 codes take
+// 41 us with 32 digits a CTA and 37 with 16; 4096 codes 22.5 with 32 and 25.7 with
+// 16, two CTAs per SM beside the scatter's.
+template <int kBins>
 __global__ void __launch_bounds__(kPrefixThreads, 8) sort_prefix_kernel(const SortArgs a) {
-  constexpr int kSplit = kPrefixThreads / kPrefixBins;
-  __shared__ int32_t s_sum[kSplit][kPrefixBins];
+  constexpr int kSplit = kPrefixThreads / kBins;
+  __shared__ int32_t s_sum[kSplit][kBins];
   sarr::dependents_may_start();
   sarr::wait_for_previous();
-  const int bins = a.bins, d = blockIdx.x * kPrefixBins + (threadIdx.x & (kPrefixBins - 1));
-  const int part = threadIdx.x / kPrefixBins, per = (a.tiles + kSplit - 1) / kSplit;
+  const int bins = a.bins, d = blockIdx.x * kBins + (threadIdx.x & (kBins - 1));
+  const int part = threadIdx.x / kBins, per = (a.tiles + kSplit - 1) / kSplit;
   const int t0 = min(part * per, a.tiles), t1 = min(t0 + per, a.tiles);
   int32_t* c = a.counts + d;
   int sum = 0;
@@ -437,13 +440,13 @@ __global__ void __launch_bounds__(kPrefixThreads, 8) sort_prefix_kernel(const So
 #pragma unroll 8
     for (int t = t0; t < t1; ++t) sum += __ldcg(c + (int64_t)t * bins);
   }
-  s_sum[part][threadIdx.x & (kPrefixBins - 1)] = sum;
+  s_sum[part][threadIdx.x & (kBins - 1)] = sum;
   __syncthreads();
   if (d >= bins) return;
   int at = 0, all = 0;
 #pragma unroll
   for (int k = 0; k < kSplit; ++k) {
-    const int x = s_sum[k][threadIdx.x & (kPrefixBins - 1)];
+    const int x = s_sum[k][threadIdx.x & (kBins - 1)];
     if (k < part) at += x;
     all += x;
   }
@@ -1036,7 +1039,8 @@ cudaError_t run_sort(SortArgs a, const SortPlan& P, char* w, int32_t* order, int
     if ((int64_t)tiles * bins > kDirectCounts) {
       a.totals = reinterpret_cast<int32_t*>(w + P.totals_at);
       sarr::count_launches(1);
-      e = sarr::launch(sort_prefix_kernel, {dim3((bins + kPrefixBins - 1) / kPrefixBins), kPrefixThreads, 0, true}, s, a);
+      e = bins <= 148 * 16 ? sarr::launch(sort_prefix_kernel<16>, {dim3((bins + 15) / 16), kPrefixThreads, 0, true}, s, a)
+                           : sarr::launch(sort_prefix_kernel<32>, {dim3((bins + 31) / 32), kPrefixThreads, 0, true}, s, a);
       if (e != cudaSuccess) return e;
     }
     e = sarr::launch(sort_scatter_kernel<kRounds>, {dim3(tiles), kSortThreads, kSmem + 4 * bins, true}, s, a);
