@@ -8,8 +8,8 @@
 //
 // The gradients of all tensors are cut into pieces of a few KB, whatever tensors
 // they belong to, and dealt to the CTAs round robin (neighbouring CTAs read
-// neighbouring pieces; a contiguous run per CTA took 5 to 10 % longer), so a list
-// of many small tensors and one flat buffer cost the same.
+// neighbouring pieces; with a contiguous run per CTA 40M parameters took 3 % longer,
+// 1M a quarter), so a list of many small tensors costs little more than one buffer.
 //
 //   norm_kernel    one partial sum (or maximum) per CTA, in 64 bits: a square
 //                  neither overflows nor underflows, and the sum keeps the
@@ -19,8 +19,10 @@
 //   clip_kernel,   every CTA adds the partials itself, in the same fixed order
 //   adam_kernel    (so that all get the same c without another launch), then
 //                  makes its elements, from the last piece down, newest in L2
-//                  first. Bound by HBM: clip_kernel 936 MB in 174 us (5.4 TB/s; two
-//                  loads a thread, 189 us with four, 182 with one), adam_kernel
+//                  first. Bound by HBM: clip_kernel 936 MB in 176 us (5.3 TB/s; two
+//                  loads a thread, 188 us with four, 172 with one, which takes longer
+//                  in place, 252 against 245 us for a norm and 160 odd tensors),
+//                  900 MB of one tensor in 160 us (5.6 TB/s), adam_kernel
 //                  1.12 GB in 168 us (6.7 TB/s; a grid of 96 CTAs per SM, 184 us
 //                  with 6).
 //
@@ -284,7 +286,10 @@ __global__ void __launch_bounds__(kThreads, 8) clip_kernel(const __grid_constant
   for (int64_t p = L.pieces - 1 - blockIdx.x; p >= 0; p -= gridDim.x) {
     while (p < first) first = first_piece(L, --t);
     const Entry& E = L.e[t];
-    if (c == 1.0f && E.out == E.in) continue;  // in place and nothing to clip: c x is x
+    if (c == 1.0f && E.out == E.in) {  // in place and nothing to clip, c x is x: on to the tensor before
+      p -= (p - first) / gridDim.x * gridDim.x;
+      continue;
+    }
     const int64_t piece = p - first;
     if (E.type == SARR_F32) piece_clip<SARR_F32, SARR_F32>(E, piece, c);
     else if (E.type == SARR_BF16 && E.out_type == SARR_BF16) piece_clip<SARR_BF16, SARR_BF16>(E, piece, c);
