@@ -153,10 +153,11 @@ def clip_grads(grads: Sequence[torch.Tensor], max_norm: float, norm_type: float 
 
 
 def clip_grad_norm_(parameters: Iterable[torch.Tensor], max_norm: float, norm_type: float = 2.0,
-                    error_if_nonfinite: bool = False) -> torch.Tensor:
+                    error_if_nonfinite: bool = False, foreach: Optional[bool] = None) -> torch.Tensor:
     """torch.nn.utils.clip_grad_norm_: clips the .grad of `parameters` (a tensor
     or several) in place and returns their total norm. error_if_nonfinite
-    reads the norm on the host before anything is clipped."""
+    reads the norm on the host before anything is clipped; foreach is accepted
+    and changes nothing (the list is always taken as one)."""
     if isinstance(parameters, torch.Tensor):
         parameters = [parameters]
     grads = [p.grad for p in parameters if p.grad is not None]

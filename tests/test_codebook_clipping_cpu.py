@@ -175,4 +175,10 @@ def test_python_refuses_cpu_tensors_and_bad_arguments():
     with pytest.raises(RuntimeError, match="CUDA"):
         clipping.adam_step_clipped(*[torch.zeros(4)] * 4, [(4, 1e-3)], 1, 1.0)
     assert clipping.grad_norm([]).item() == 0.0
-    assert clipping.clip_grad_norm_([torch.zeros(3, requires_grad=True)], 1.0).item() == 0.0
+    assert clipping.clip_grad_norm_([torch.zeros(3, requires_grad=True)], 1.0, foreach=True).item() == 0.0
+
+
+def test_clip_grad_norm_takes_torchs_arguments():
+    import inspect
+    mine = inspect.signature(clipping.clip_grad_norm_).parameters
+    assert list(inspect.signature(torch.nn.utils.clip_grad_norm_).parameters) == list(mine)
