@@ -6,7 +6,6 @@ form (elementary torch operations) or, where `own` is true, through
 and at most 2M Gaussians of 3 + 3 + 4 + 1 + 16 floats, 16 SH coefficients) and
 generic embedding tables.
 """
-import functools
 import math
 import os
 import sys
@@ -22,7 +21,6 @@ SIZE = {"f32": 4, "bf16": 2, "f16": 2, "i32": 4, "i64": 8}
 BETA1, BETA2, EPS = 0.9, 0.999, 1e-8
 
 
-@functools.lru_cache(maxsize=1)
 def _package():
     root = os.path.join(os.getcwd(), "sar-3dgs_b200")
     if root not in sys.path:
