@@ -20,6 +20,7 @@ import functools
 from typing import NamedTuple, Optional
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _native
@@ -224,10 +225,12 @@ def lookup(table: torch.Tensor, index: torch.Tensor, scale: float = 1.0,
     index[i] is outside [0, codes)), in `dtype` (the table's type by default, or
     float32), with its gradient with respect to the table. `order`: what
     sort_by_code gave for this index, where the caller keeps it; without it the
-    gradient sorts the index."""
+    gradient sorts the index. Forward-mode differentiation is refused."""
     if order is not None and (order.order.numel() != index.numel() or order.offsets.numel() != table.shape[0] + 1):
         raise RuntimeError(f"order is of {order.order.numel()} Gaussians and {order.offsets.numel() - 1} codes, the "
                            f"index of {index.numel()} and the table of {table.shape[0]}")
-    if isinstance(table, torch.Tensor) and table.requires_grad and torch.is_grad_enabled():
+    # a dual table need not require a gradient; apply refuses it
+    if isinstance(table, torch.Tensor) and (table.requires_grad and torch.is_grad_enabled()
+                                            or forward_ad.unpack_dual(table).tangent is not None):
         return _Lookup.apply(table, index, scale, dtype, order)
     return _lookup(table, index, scale, dtype)
