@@ -9,7 +9,9 @@ with torch.nn.utils.clip_grad_norm_'s rule: every gradient is multiplied by
 min(1, max_norm / (norm + 1e-6)). Gradients are dense float32, bfloat16 or
 float16 CUDA tensors of one device, types mixed as they come; the norm is summed
 in 64 bits and returned as a float32 scalar on the device (no synchronisation).
-Results are bitwise reproducible. The reference trains without clipping.
+Results are bitwise reproducible. A tensor written in place is a new version for
+autograd, as with torch's in-place operations: a graph that saved it refuses its
+backward. The reference trains without clipping.
 """
 import ctypes
 import functools
@@ -19,6 +21,7 @@ from operator import attrgetter
 from typing import Iterable, Optional, Sequence
 
 import torch
+from torch.autograd.graph import increment_version
 
 from . import _native
 
@@ -149,6 +152,7 @@ def clip_grads(grads: Sequence[torch.Tensor], max_norm: float, norm_type: float 
             len(grads), _at(ptrs), _at(counts), _at(types), _at(optrs), _at(otypes), kind,
             float(max_norm), norm.data_ptr(), ws.data_ptr(), ws.numel(), _native._raw_stream(dev)),
             "sarr_clip_grads")
+    increment_version(grads if out is None else out)
     return norm
 
 
@@ -207,3 +211,4 @@ def adam_ranges_clipped(tensors, ranges, step, max_norm, betas, eps, norm, ws):
         len(ranges), _at(begin), _at(end), _at(first), _at(lr), *[t.data_ptr() for t in tensors],
         float(betas[0]), float(betas[1]), float(eps), int(step), float(max_norm), norm.data_ptr(),
         ws.data_ptr(), ws.numel(), _native._raw_stream(tensors[0].device)), "sarr_adam_step_clipped")
+    increment_version((tensors[0], tensors[2], tensors[3], norm))

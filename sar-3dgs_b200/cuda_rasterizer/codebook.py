@@ -22,6 +22,7 @@ from typing import NamedTuple, Optional
 import torch
 from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
+from torch.autograd.graph import increment_version
 
 from . import _native
 
@@ -111,6 +112,8 @@ def _lookup(table, index, scale, dtype, out=None):
             n, codes, cols, index.data_ptr(), _INDEX_BITS[index.dtype], table.data_ptr(),
             _TYPES[table.dtype], stride, float(scale), rows.data_ptr(), _TYPES[dtype], rows_stride,
             _native._raw_stream(dev)), "sarr_codebook_lookup")
+    if out is not None:
+        increment_version(out)
     return rows
 
 
@@ -168,6 +171,8 @@ def gradient_sorted(grad_rows: torch.Tensor, sorted_codes: SortedCodes, scale: f
             n, codes, cols, rows.data_ptr(), _TYPES[rows.dtype], rows_stride, order.data_ptr(),
             places.data_ptr(), offsets.data_ptr(), float(scale), table.data_ptr(), _TYPES[dtype], stride,
             ws.data_ptr(), size, _native._raw_stream(dev)), "sarr_codebook_grad")
+    if out is not None:
+        increment_version(out)
     return table
 
 
