@@ -245,7 +245,10 @@ int sarr_codebook_sort(int64_t n, int64_t codes, const void *index, int index_bi
  *   grad_rows [n, cols] in rows_type; grad_table [codes, cols] in table_type
  *   (the types are equal or one of them is SARR_F32), both with a row stride in
  *   elements >= cols. Sums are kept in 32 bits and rounded once, in an order
- *   that depends on the sizes and the codes only, so the result is reproducible.
+ *   that depends on the sizes, the codes, the types, the strides and the offsets
+ *   of grad_rows and grad_table from a 16-byte boundary (which set the width of
+ *   the accesses, and with it how the sums are cut): with these equal, the bits
+ *   are equal.
  *   order, sorted_codes and offsets must be what sarr_codebook_sort wrote for
  *   the same n and codes; order and sorted_codes 16-byte aligned.
  */
@@ -275,7 +278,9 @@ int sarr_codebook_gradient(int64_t n, int64_t codes, int64_t cols, const void *g
  * float on the device). grads, counts and types are host arrays: the device
  * pointer, the number of elements (contiguous memory) and the SARR_F32 /
  * SARR_BF16 / SARR_F16 type of each tensor; types may be mixed. Squares are
- * summed in 64 bits (no overflow or underflow of a square) in a fixed order.
+ * summed in 64 bits (no overflow or underflow of a square) in an order that
+ * depends on the counts, the types and each tensor's offset from a 16-byte
+ * boundary: with these equal, the bits are equal.
  * A NaN anywhere makes the norm NaN. An empty list has norm 0. Workspace:
  * sarr_grad_norm_workspace_size. No reference counterpart (the reference
  * trains without clipping).

@@ -9,7 +9,11 @@
 //             i with index[i] = c, zeros for a code that none has
 //
 // Sums are in 32 bits and in a fixed order (the sort is stable and nothing is
-// added by atomics), so the same inputs give the same bits.
+// added by atomics): the same inputs at the same offsets from a 16-byte boundary
+// give the same bits. Rows that are not aligned are read in narrower vectors, which
+// cut the sums into other parts; parts that do not depend on the alignment were
+// tried, and made such rows slower (16,381 of 1024 bf16, one element behind a
+// boundary: 65 to 114 us against 61).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <stdint.h>

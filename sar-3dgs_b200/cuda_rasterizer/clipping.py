@@ -9,7 +9,8 @@ with torch.nn.utils.clip_grad_norm_'s rule: every gradient is multiplied by
 min(1, max_norm / (norm + 1e-6)). Gradients are dense float32, bfloat16 or
 float16 CUDA tensors of one device, types mixed as they come; the norm is summed
 in 64 bits and returned as a float32 scalar on the device (no synchronisation).
-Results are bitwise reproducible. A tensor written in place is a new version for
+Results are bitwise reproducible for tensors at the same offsets from a 16-byte
+boundary. A tensor written in place is a new version for
 autograd, as with torch's in-place operations: a graph that saved it refuses its
 backward. The reference trains without clipping.
 """

@@ -12,8 +12,10 @@ is zeros and its gradient reaches no code.
 
 Tables and rows are float32, bfloat16 or float16 CUDA tensors (rows in the
 table's type or float32); indexes int32 or int64. Products and sums are formed
-in 32 bits and rounded once; results are bitwise reproducible. No counterpart
-in the reference, which keeps all SH coefficients of every Gaussian.
+in 32 bits and rounded once. Results are bitwise reproducible: a gradient's bits
+depend on the sizes, codes, types and strides and on the rows' and the table's
+offsets from a 16-byte boundary. No counterpart in the reference, which keeps all
+SH coefficients of every Gaussian.
 """
 import ctypes
 import functools
