@@ -249,6 +249,7 @@ int sarr_codebook_sort(int64_t n, int64_t codes, const void *index, int index_bi
  *   of grad_rows and grad_table from a 16-byte boundary (which set the width of
  *   the accesses, and with it how the sums are cut): with these equal, the bits
  *   are equal.
+ *   grad_table must not overlap what is read.
  *   order, sorted_codes and offsets must be what sarr_codebook_sort wrote for
  *   the same n and codes; order and sorted_codes 16-byte aligned.
  */
@@ -313,8 +314,9 @@ int sarr_clip_grads(int n_tensors, const void *const *grads, const int64_t *coun
  * with c * g in the place of the gradient g (c as in sarr_clip_grads; the
  * gradients are not rewritten). Up to 64 disjoint ranges (host arrays as in
  * sarr_adam_step_ranges, range_lr in double); betas, eps and learning rates in
- * double as torch holds them. norm_out (device float) may be NULL. Workspace:
- * sarr_grad_norm_workspace_size(64).
+ * double as torch holds them. The ranges of param, exp_avg and exp_avg_sq must
+ * not overlap one another or the gradients'. norm_out (device float) may be
+ * NULL. Workspace: sarr_grad_norm_workspace_size(64).
  */
 int sarr_adam_step_clipped(int n_ranges, const int64_t *range_begin, const int64_t *range_end,
                            const int64_t *grad_begin, const double *range_lr, float *param,

@@ -176,16 +176,19 @@ def clip_grad_norm_(parameters: Iterable[torch.Tensor], max_norm: float, norm_ty
 
 def adam_step_clipped(param, grad, exp_avg, exp_avg_sq, segments, step, max_norm, betas=(0.9, 0.999),
                       eps=1e-8) -> torch.Tensor:
-    """torch.optim.Adam's update over flat float32 buffers of equal length with
-    the gradient clipped by its 2-norm (the gradient itself is not rewritten);
-    `segments` = [(end, lr), ...] with ascending ends that cover the buffers, as
-    in _native.adam_step; `step` counts from 1. Returns the norm."""
+    """torch.optim.Adam's update over flat float32 buffers of equal length (which
+    share no memory) with the gradient clipped by its 2-norm (the gradient itself
+    is not rewritten); `segments` = [(end, lr), ...] with ascending ends that cover
+    the buffers, as in _native.adam_step; `step` counts from 1. Returns the norm."""
     tensors = (param, grad, exp_avg, exp_avg_sq)
     for t, name in zip(tensors, ("param", "grad", "exp_avg", "exp_avg_sq")):
         _native._as_cuda_f32(t, name)
         if t.numel() != param.numel() or not t.is_contiguous() or t.device != param.device:
             raise RuntimeError("Adam buffers must be contiguous, of equal length and on one device")
     count, dev = param.numel(), param.device
+    places = sorted(map(torch.Tensor.data_ptr, tensors))
+    if any(b - a < 4 * count for a, b in zip(places, places[1:])):
+        raise RuntimeError("Adam buffers must not share memory")
     ranges, at = [], 0
     for end, lr in segments:
         ranges.append((at, int(end), at, lr))

@@ -87,6 +87,22 @@ def _check_out(out, rows, cols, dev, name="out"):
     return stride
 
 
+def _meet(a, a_stride, b, b_stride):
+    """Whether two matrices with contiguous rows (strides in elements) share memory."""
+    if not (a.numel() and b.numel()):
+        return False
+    (n, a_cols), (m, b_cols) = a.shape, b.shape
+    a_size, b_size, at = a.element_size(), b.element_size(), b.data_ptr() - a.data_ptr()
+    a_cols, b_cols, a_pitch, b_pitch = a_cols * a_size, b_cols * b_size, a_stride * a_size, b_stride * b_size
+    if at >= (n - 1) * a_pitch + a_cols or -at >= (m - 1) * b_pitch + b_cols:
+        return False
+    # side by side in rows of one pitch (a single row has that of the other)
+    pitch = b_pitch if n == 1 else a_pitch
+    if m > 1 and b_pitch != pitch:
+        return True
+    return at % pitch < a_cols or at % pitch + b_cols > pitch
+
+
 @functools.lru_cache(maxsize=1024)
 def _size(name, *args):
     """Workspace bytes for these sizes."""
@@ -146,7 +162,8 @@ def gradient_sorted(grad_rows: torch.Tensor, sorted_codes: SortedCodes, scale: f
     """The table's gradient [codes, cols] from the rows' gradients [n, cols] and
     the order that sort_by_code gave for their index. `dtype`: the result's type
     (the rows' type by default; float32, or any of the three for float32 rows);
-    `out`: a matrix to write it into (its rows may be strided)."""
+    `out`: a matrix to write it into (its rows may be strided; it shares no memory
+    with the other arguments)."""
     rows, rows_stride = _matrix(grad_rows, "grad_rows")
     n, cols = rows.shape
     order, places, offsets = sorted_codes
@@ -163,6 +180,9 @@ def gradient_sorted(grad_rows: torch.Tensor, sorted_codes: SortedCodes, scale: f
         stride = _check_out(out, codes, cols, dev)
         if dtype is not None and dtype != out.dtype:
             raise RuntimeError(f"out is {out.dtype}, dtype {dtype}")
+        if _meet(out, stride, rows, rows_stride) or any(
+                _meet(out, stride, t.unsqueeze(0), t.numel()) for t in (order, places, offsets)):
+            raise RuntimeError("out must not share memory with grad_rows or sorted_codes")
         dtype = out.dtype
     dtype = _gradient_type(rows, dtype)
     size = _size("sarr_codebook_grad_workspace_size", n, cols)
