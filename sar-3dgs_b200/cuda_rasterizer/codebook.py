@@ -253,9 +253,15 @@ def lookup(table: torch.Tensor, index: torch.Tensor, scale: float = 1.0,
     float32), with its gradient with respect to the table. `order`: what
     sort_by_code gave for this index, where the caller keeps it; without it the
     gradient sorts the index. Forward-mode differentiation is refused."""
-    if order is not None and (order.order.numel() != index.numel() or order.offsets.numel() != table.shape[0] + 1):
-        raise RuntimeError(f"order is of {order.order.numel()} Gaussians and {order.offsets.numel() - 1} codes, the "
-                           f"index of {index.numel()} and the table of {table.shape[0]}")
+    if order is not None:
+        for t, name in ((table, "table"), (index, "index")):
+            if not isinstance(t, torch.Tensor):
+                raise TypeError(f"{name} must be a torch.Tensor")
+        if not isinstance(order, SortedCodes) or not all(isinstance(t, torch.Tensor) for t in order):
+            raise TypeError("order must be what sort_by_code gave")
+        if table.dim() == 2 and (order.order.numel() != index.numel() or order.offsets.numel() != table.shape[0] + 1):
+            raise RuntimeError(f"order is of {order.order.numel()} Gaussians and {order.offsets.numel() - 1} codes, "
+                               f"the index of {index.numel()} and the table of {table.shape[0]}")
     # a dual table need not require a gradient; apply refuses it
     if isinstance(table, torch.Tensor) and (table.requires_grad and torch.is_grad_enabled()
                                             or forward_ad.unpack_dual(table).tangent is not None):

@@ -64,3 +64,15 @@ def test_adam_buffers_that_overlap_are_refused(no_kernels):
             clipping.adam_step_clipped(*bad, [(16, 1e-3)], 1, 1.0)
     e = memory[:0]
     clipping.adam_step_clipped(e, e, e, e, [(0, 1e-3)], 1, 1.0)
+
+
+def test_lookup_with_something_else_as_order():
+    table, index = torch.ones(4, 3), torch.zeros(5, dtype=torch.int64)
+    for bad in (tuple(_order(5, 4)), torch.zeros(5, dtype=torch.int32), codebook.SortedCodes(None, None, None)):
+        with pytest.raises(TypeError, match="order"):
+            codebook.lookup(table, index, order=bad)
+    for bad in ([[1.0]], None):
+        with pytest.raises(TypeError):
+            codebook.lookup(bad, index, order=_order(5, 4))
+        with pytest.raises(TypeError):
+            codebook.lookup(table, bad, order=_order(5, 4))
