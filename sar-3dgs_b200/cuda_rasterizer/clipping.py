@@ -52,7 +52,7 @@ def _list(tensors, name):
         n, dtypes, dev = len(tensors), list(map(_DTYPE, tensors)), tensors[0].device
         contiguous = all(map(torch.Tensor.is_contiguous, tensors))
         if (dev.type == "cuda" and list(map(torch.Tensor.get_device, tensors)).count(dev.index) == n
-                and (contiguous or all(map(_dense, tensors)))):
+                and (contiguous or all(map(_dense, tensors))) and not any(map(torch.Tensor.is_neg, tensors))):
             if dtypes.count(dtypes[0]) == n:
                 types = array("i", [_TYPES[dtypes[0]]]) * n
             else:
@@ -74,6 +74,8 @@ def _list(tensors, name):
         dev = t.device
         if not _dense(t):
             raise RuntimeError(f"{name}[{k}] must be dense, got shape {tuple(t.shape)} with strides {t.stride()}")
+        if t.is_neg():
+            raise RuntimeError(f"{name}[{k}] is a negated view (resolve_neg makes a tensor of it)")
     raise RuntimeError(f"{name} cannot be used")
 
 

@@ -51,6 +51,7 @@ def _matrix(t, name):
         raise RuntimeError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
     if t.dim() != 2:
         raise RuntimeError(f"{name} must be a matrix, got shape {tuple(t.shape)}")
+    t = t.resolve_neg()
     rows, cols = t.shape
     stride, step = t.stride()
     if (cols > 1 and step != 1) or (rows > 1 and stride < cols):

@@ -76,3 +76,18 @@ def test_lookup_with_something_else_as_order():
             codebook.lookup(bad, index, order=_order(5, 4))
         with pytest.raises(TypeError):
             codebook.lookup(table, bad, order=_order(5, 4))
+
+
+def test_negated_views(monkeypatch):
+    """The imaginary part of a conjugate is a view whose memory holds the values negated."""
+    monkeypatch.setattr(torch.Tensor, "is_cuda", True)
+    z = torch.complex(torch.ones(4, 1), torch.full((4, 1), 2.0)).conj().imag
+    assert z.is_neg()
+    t, stride = codebook._matrix(z, "table")
+    assert not t.is_neg() and torch.equal(t, torch.full((4, 1), -2.0)) and stride == 1
+    with pytest.raises(RuntimeError, match="out"):
+        codebook._check_out(z, 4, 1, z.device)
+    plain = torch.ones(4, 6)[:, :3]
+    assert codebook._matrix(plain, "table")[0] is plain
+    with pytest.raises(RuntimeError, match="negated"):
+        clipping._list([torch.ones(1), z[0]], "grads")
