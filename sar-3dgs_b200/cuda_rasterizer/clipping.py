@@ -52,7 +52,7 @@ def _list(tensors, name):
         n, dtypes, dev = len(tensors), list(map(_DTYPE, tensors)), tensors[0].device
         contiguous = all(map(torch.Tensor.is_contiguous, tensors))
         if (dev.type == "cuda" and list(map(torch.Tensor.get_device, tensors)).count(dev.index) == n
-                and (contiguous or all(map(_dense, tensors))) and not any(map(torch.Tensor.is_neg, tensors))):
+                and (contiguous or all(map(_dense, tensors)))):
             if dtypes.count(dtypes[0]) == n:
                 types = array("i", [_TYPES[dtypes[0]]]) * n
             else:
@@ -74,8 +74,6 @@ def _list(tensors, name):
         dev = t.device
         if not _dense(t):
             raise RuntimeError(f"{name}[{k}] must be dense, got shape {tuple(t.shape)} with strides {t.stride()}")
-        if t.is_neg():
-            raise RuntimeError(f"{name}[{k}] is a negated view (resolve_neg makes a tensor of it)")
     raise RuntimeError(f"{name} cannot be used")
 
 
@@ -138,6 +136,9 @@ def clip_grads(grads: Sequence[torch.Tensor], max_norm: float, norm_type: float 
     optrs, otypes = ptrs, types
     if out is not None:
         optrs, ocounts, otypes, odev, oflat = _list(out, "out")
+        # (in place a view of negated values is scaled as any other)
+        if any(map(torch.Tensor.is_neg, grads)) or any(map(torch.Tensor.is_neg, out)):
+            raise RuntimeError("grads or out has a negated view (resolve_neg makes a tensor of it)")
         if ocounts != counts or odev != dev:
             raise RuntimeError("out must have the gradients' sizes and device")
         if otypes != types:
@@ -188,8 +189,8 @@ def adam_step_clipped(param, grad, exp_avg, exp_avg_sq, segments, step, max_norm
         if t.numel() != param.numel() or not t.is_contiguous() or t.device != param.device:
             raise RuntimeError("Adam buffers must be contiguous, of equal length and on one device")
     count, dev = param.numel(), param.device
-    places = sorted(map(torch.Tensor.data_ptr, tensors))
-    if any(b - a < 4 * count for a, b in zip(places, places[1:])):
+    a, b, c, d = sorted(map(torch.Tensor.data_ptr, tensors))
+    if min(b - a, c - b, d - c) < 4 * count:
         raise RuntimeError("Adam buffers must not share memory")
     ranges, at = [], 0
     for end, lr in segments:

@@ -89,19 +89,24 @@ def _check_out(out, rows, cols, dev, name="out"):
 
 
 def _meet(a, a_stride, b, b_stride):
-    """Whether two matrices with contiguous rows (strides in elements) share memory."""
-    if not (a.numel() and b.numel()):
+    """Whether a matrix with contiguous rows (stride in elements) shares memory with
+    another, or with a vector."""
+    at = b.data_ptr() - a.data_ptr()
+    n, cols = a.shape
+    a_size = a.element_size()
+    if at >= ((n - 1) * a_stride + cols) * a_size:  # the usual answers
         return False
-    (n, a_cols), (m, b_cols) = a.shape, b.shape
-    a_size, b_size, at = a.element_size(), b.element_size(), b.data_ptr() - a.data_ptr()
-    a_cols, b_cols, a_pitch, b_pitch = a_cols * a_size, b_cols * b_size, a_stride * a_size, b_stride * b_size
-    if at >= (n - 1) * a_pitch + a_cols or -at >= (m - 1) * b_pitch + b_cols:
+    m, b_cols = b.shape if b.dim() == 2 else (1, b.numel())
+    b_size = b.element_size()
+    if -at >= ((m - 1) * b_stride + b_cols) * b_size or not (n and cols and m and b_cols):
         return False
     # side by side in rows of one pitch (a single row has that of the other)
-    pitch = b_pitch if n == 1 else a_pitch
-    if m > 1 and b_pitch != pitch:
+    pitch = b_stride * b_size if n == 1 else a_stride * a_size
+    if m > 1 and b_stride * b_size != pitch:
         return True
-    return at % pitch < a_cols or at % pitch + b_cols > pitch
+    if n == 1 and m == 1:
+        return True
+    return at % pitch < cols * a_size or at % pitch + b_cols * b_size > pitch
 
 
 @functools.lru_cache(maxsize=1024)
@@ -181,8 +186,8 @@ def gradient_sorted(grad_rows: torch.Tensor, sorted_codes: SortedCodes, scale: f
         stride = _check_out(out, codes, cols, dev)
         if dtype is not None and dtype != out.dtype:
             raise RuntimeError(f"out is {out.dtype}, dtype {dtype}")
-        if _meet(out, stride, rows, rows_stride) or any(
-                _meet(out, stride, t.unsqueeze(0), t.numel()) for t in (order, places, offsets)):
+        if _meet(out, stride, rows, rows_stride) or any([
+                _meet(out, stride, t, 0) for t in (order, places, offsets)]):
             raise RuntimeError("out must not share memory with grad_rows or sorted_codes")
         dtype = out.dtype
     dtype = _gradient_type(rows, dtype)

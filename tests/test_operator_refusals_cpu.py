@@ -1,6 +1,7 @@
 """Calls of the codebook and clipping operators that are refused before a kernel runs,
 without a GPU: the host side of the calls, with the kernel call replaced by nothing."""
 import contextlib
+from array import array
 
 import pytest
 import torch
@@ -89,5 +90,16 @@ def test_negated_views(monkeypatch):
         codebook._check_out(z, 4, 1, z.device)
     plain = torch.ones(4, 6)[:, :3]
     assert codebook._matrix(plain, "table")[0] is plain
-    with pytest.raises(RuntimeError, match="negated"):
-        clipping._list([torch.ones(1), z[0]], "grads")
+
+
+def test_negated_views_in_lists(no_kernels, monkeypatch):
+    """In place the values are scaled as they lie; into others the sign would be lost."""
+    monkeypatch.setattr(clipping, "_list", lambda tensors, name: (
+        array("Q", [t.data_ptr() for t in tensors]), array("q", [t.numel() for t in tensors]),
+        array("i", [0] * len(tensors)), tensors[0].device, True))
+    z = torch.complex(torch.ones(1), torch.ones(1)).conj().imag
+    assert z.is_neg() and z.is_contiguous()
+    clipping.clip_grads([torch.ones(1), z], 1.0)
+    for grads, out in (([z], [torch.ones(1)]), ([torch.ones(1)], [z])):
+        with pytest.raises(RuntimeError, match="negated"):
+            clipping.clip_grads(grads, 1.0, out=out)
