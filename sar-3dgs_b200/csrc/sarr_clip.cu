@@ -14,15 +14,16 @@
 //   norm_kernel    one partial sum (or maximum) per CTA, in 64 bits: a square
 //                  neither overflows nor underflows, and the sum keeps the
 //                  accuracy of its terms; written to the workspace in CTA order.
-//                  At the copy rate: 468 MB in 74 us (6.3 TB/s);
+//                  At the copy rate: 468 MB in 74 us (6.3 TB/s); the largest
+//                  magnitude in 100 (two 64-bit compares an element);
 //   finish_kernel  adds the partials and writes N (norm only);
 //   clip_kernel,   every CTA adds the partials itself, in the same fixed order
 //   adam_kernel    (so that all get the same c without another launch), then
 //                  makes its elements, from the last piece down, newest in L2
-//                  first. Bound by HBM: clip_kernel 936 MB in 176 us (5.3 TB/s; two
-//                  loads a thread, 188 us with four, 172 with one, which takes longer
-//                  in place, 252 against 245 us for a norm and 160 odd tensors),
-//                  900 MB of one tensor in 160 us (5.6 TB/s), adam_kernel
+//                  first. Bound by HBM: clip_kernel 936 MB in 172 us (5.4 TB/s; with
+//                  two loads a thread norm and clip of 160 odd tensors take 243 us
+//                  into others and 248 in place, with one 239 and 251),
+//                  900 MB of one tensor in 151 us (6.0 TB/s), adam_kernel
 //                  1.12 GB in 168 us (6.7 TB/s; a grid of 96 CTAs per SM, 184 us
 //                  with 6).
 //

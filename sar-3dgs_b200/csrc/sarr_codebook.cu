@@ -139,6 +139,9 @@ __device__ __forceinline__ uint32_t code_of(const void* index, bool wide, int64_
 // rows of 1000 bf16 11.9 us (5.5 TB/s). Six rows a thread and CTAs of 64 threads:
 // 12.9 us against 14.1 with 4 and 256 and 15.6 with 8 and 256 (short CTAs fill the
 // tail), 27 where a lane wrote 32 bytes in two halves; 1000 rows take 2 us, a launch.
+// Columns that are no whole number of vectors are read and written one or two at a
+// time: 1M rows of 3 floats take 8.6 us (16 MB), the first 9 of 16 columns 42 (rows
+// of 64 bytes written in part), the first 4 13.5.
 constexpr int kLookupThreads = 64;
 constexpr int kLookupRows = 6;  // rows per thread, their loads in flight together
 
@@ -577,15 +580,21 @@ __global__ void __launch_bounds__(256) sort_offsets_kernel(int n, uint32_t codes
 // others wait for their rows (evenly among them they hold the spans up: 39 us
 // against 31 for 16,381 rows of 1024 bf16 into 32,000).
 //
-// Bound by the rows' reads. Rows of 1024 bf16: 31 us for 165 MB (5.3 TB/s, 0.81 of
-// the measured copy bandwidth). Rows of 16 floats come as random 64-byte reads: 1M
-// of them 20.6 us (24 where one code has 6 % of them), and the lookup kernel reads
-// 64 MB of random rows in about 20 us too; taken in the order of the sort there is
-// nothing to stream.
+// Rows of 1024 bf16 are bound by their reads: 31 us for 165 MB (5.3 TB/s, 0.81 of
+// the measured copy bandwidth). Rows of 16 floats are bound by latency: 1M of them
+// take 20.6 us for 72 MB from HBM, 24 where one code has 6 % of them and 26 where one
+// has all (14, 16 and 19 with the rows in L2). With one code the rows are read one
+// after another, so it is not their random places: there is one wave of CTAs, each
+// of which waits for its codes and its order, then loads eight rows when the eight
+// before are added; a code over all spans has its 489 partials added by one CTA.
 constexpr int kGradThreads = 256;
 constexpr int kGradRows = 8;     // rows of a group loaded together
 constexpr int kMaxPart = 64;     // places of a group, at most; a multiple of kGradRows
-constexpr int kOneSpanPart = 16;  // places of a group up to which one CTA takes them all
+// Places of a group up to which one CTA takes them all, without a kernel behind it:
+// 1000 rows of 16 4.5 us against 5.5 in several, 2048 of 8 5.4 against 6.2, 256 of 64
+// 3.8 against 4.1. With up to 32 places 2048 rows of 16 take 6.4 us in one CTA against
+// 5.9 in several, 4096 of 8 7.7 against 6.4, 512 of 64 5.6 against 5.0.
+constexpr int kOneSpanPart = 16;
 constexpr int kMaxSpan = 2048;   // places of a CTA, at most
 constexpr int kFinishThreads = 64;
 constexpr int kFillCodes = 8;    // codes of a group in a zero-writing CTA
@@ -1072,8 +1081,6 @@ GradPlan grad_plan(int64_t n, int64_t cols, int v) {
   P.lanes = pow2_at_least(vecs, kGradThreads);
   P.tiles = (vecs + P.lanes - 1) / P.lanes;
   const int64_t groups = kGradThreads / P.lanes, spans = std::max<int64_t>(grad_ctas(v) / P.tiles, 1);
-  // few rows: all in one span, which needs no kernel behind it (1000 rows of 16
-  // with their sort: 8.9 -> 7.9 us)
   const bool one = n <= groups * kOneSpanPart;
   const int64_t share = (n + groups * (one ? 1 : spans) - 1) / (groups * (one ? 1 : spans)), most = std::min<int64_t>(kMaxPart, kMaxSpan / groups);
   P.part = (int)std::max<int64_t>(std::min((share + kGradRows - 1) / kGradRows * kGradRows, most), kGradRows);
